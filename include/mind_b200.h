@@ -94,6 +94,64 @@ int64_t __mind_blas_dot_i16_v(int64_t a, int64_t b, int64_t len);
  * un-transposed K x N B, the layout of its int8 and Q16.16 GEMMs.  New symbol name. */
 int64_t __mind_b200_matmul_mm_i16(int64_t a, int64_t b, int64_t c, int64_t m, int64_t k, int64_t n);
 
+/* ---- products of quantised language models ------------------------------------------------
+ * No counterpart in the reference.  Like everything here they are exact integer arithmetic, so
+ * their bytes depend on nothing but the operands.  Calls run on the current device (host operands
+ * are staged; they are not spread over several GPUs).  Outputs must not overlap inputs.
+ *
+ * expert_plan groups the routed slots of a batch by expert.  ids: int32[count], the experts of
+ * every token, `per` of each token in a row.  With the kept slots (0 <= ids[i] < experts) sorted by
+ * (ids[i], i) and numbered p = 0, 1, ...:
+ *   offsets[e] = number of kept slots of experts below e          int32[experts + 1]
+ *   rows[p]    = i / per, the token of the slot                   int32[count]
+ *   place[i]   = p, or -1 where ids[i] names no expert            int32[count]
+ * Any other id (-1 by custom) is padding.  rows[offsets[experts]] and beyond are left as they were.
+ * count == 0 writes offsets alone.  experts is 1..4096.
+ *
+ * matmul_grouped_i8 multiplies the grouped rows by their expert's matrix: for p in
+ * [offsets[e], offsets[e + 1])
+ *   acc    = (i32) sum_k (i64)A[r,k] * (i64)B[e][k,n]    r = rows[p], or p where rows is 0
+ *   C[p,n] = acc                                          scale = 0
+ *   C[p,n] = (i32)( ((i64)acc * scale[e,n]) >> shift )    int32 scale[experts][n], shift 0..62
+ * a: a_rows x k int8 (a_rows == m where rows is 0); b: experts x k x n int8, for the _bt form
+ * experts x n x k; c: m x n int32.  rows of A outside [0, a_rows) count as zeros.  Rows of C that
+ * belong to no expert are left as they were.  offsets is int32[experts + 1], a running sum within
+ * [0, m]; a host array that is not one is refused, in device memory each bound is taken no lower
+ * than the one before and no higher than m.
+ *
+ * gemv_w4_* multiply 4-bit weights by a few tokens' activations (int8, int16 or Q16.16):
+ *   y[t,r] = (i32)( ( sum_g (i64)scale[r,g] * sum_{k in g} W[r,k] * x[t,k] ) >> shift )
+ * The sum is taken mod 2^64, shifted (arithmetic, 0..62) and truncated once.  W[r,k] is a signed
+ * 4-bit number, two a byte, the even k in the low half, rows of ceil(cols / 2) bytes; group g is
+ * columns [g * group, (g + 1) * group), group a positive multiple of 32; scale is
+ * int16[rows][ceil(cols / group)].  Scales s are stored as multiples of 2^-f for an f of the
+ * caller's: with x in units of 2^-h, y is in units of 2^-(h + f - shift).
+ * x: tokens x cols, y: tokens x rows int32.  The _grouped forms have one matrix per expert (w:
+ * experts x rows x ceil(cols / 2), scale: experts x rows x groups), m output rows grouped by
+ * `offsets`, and read row rows_of[p] of x (x_rows x cols) for output row p, or row p where rows_of
+ * is 0; offsets, rows_of and untouched rows are as for matmul_grouped_i8. */
+int64_t __mind_b200_expert_plan(int64_t ids, int64_t offsets, int64_t rows, int64_t place, int64_t count,
+                                int64_t experts, int64_t per);
+int64_t __mind_b200_matmul_grouped_i8(int64_t a, int64_t rows, int64_t b, int64_t offsets, int64_t scale, int64_t c,
+                                      int64_t m, int64_t k, int64_t n, int64_t experts, int64_t a_rows, int64_t shift);
+int64_t __mind_b200_matmul_grouped_i8_bt(int64_t a, int64_t rows, int64_t bt, int64_t offsets, int64_t scale, int64_t c,
+                                         int64_t m, int64_t k, int64_t n, int64_t experts, int64_t a_rows, int64_t shift);
+int64_t __mind_b200_gemv_w4_i8(int64_t w, int64_t scale, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols,
+                               int64_t group, int64_t shift);
+int64_t __mind_b200_gemv_w4_i16(int64_t w, int64_t scale, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols,
+                                int64_t group, int64_t shift);
+int64_t __mind_b200_gemv_w4_q16(int64_t w, int64_t scale, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols,
+                                int64_t group, int64_t shift);
+int64_t __mind_b200_gemv_w4_grouped_i8(int64_t w, int64_t scale, int64_t x, int64_t rows_of, int64_t offsets, int64_t y,
+                                       int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t shift,
+                                       int64_t experts, int64_t x_rows);
+int64_t __mind_b200_gemv_w4_grouped_i16(int64_t w, int64_t scale, int64_t x, int64_t rows_of, int64_t offsets, int64_t y,
+                                        int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t shift,
+                                        int64_t experts, int64_t x_rows);
+int64_t __mind_b200_gemv_w4_grouped_q16(int64_t w, int64_t scale, int64_t x, int64_t rows_of, int64_t offsets, int64_t y,
+                                        int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t shift,
+                                        int64_t experts, int64_t x_rows);
+
 /* ---- int8 GEMM that allocates nothing -----------------------------------------------------------
  * This entry point has no counterpart in the reference.  It is for hosts that cannot call
  * cudaMalloc when they need the product: a serving loop in which an allocation (and the device

@@ -44,9 +44,14 @@ def lib() -> C.CDLL:
                "mind_b200_lcg_fill", "mind_b200_matvec_wrap"]
         five = ["__mind_blas_gemv_q16_mt", "__mind_blas_matmul_rmajor_q16_v",
                 "__mind_blas_matmul_rmajor_i16_v", "mmq", "mmi16", "gemvq"]
+        thirteen = ["__mind_b200_gemv_w4_grouped_i8", "__mind_b200_gemv_w4_grouped_i16",
+                    "__mind_b200_gemv_w4_grouped_q16"]
+        twelve = ["__mind_b200_matmul_grouped_i8", "__mind_b200_matmul_grouped_i8_bt"]
+        nine = ["__mind_b200_gemv_w4_i8", "__mind_b200_gemv_w4_i16", "__mind_b200_gemv_w4_q16"]
+        seven = ["__mind_b200_expert_plan"]
         three = ["__mind_blas_dot_q16_v", "__mind_blas_dot_l1_q16_v", "__mind_blas_dot_i16_v",
                  "dotq", "dotl1q", "doti16"]
-        for names, n in ((six, 6), (five, 5), (three, 3)):
+        for names, n in ((thirteen, 13), (twelve, 12), (nine, 9), (seven, 7), (six, 6), (five, 5), (three, 3)):
             for name in names:
                 f = getattr(L, name)
                 f.argtypes, f.restype = [i64] * n, i64

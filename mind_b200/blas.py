@@ -89,6 +89,72 @@ def dot_i16_v(a, b, n):
     return _dot("__mind_blas_dot_i16_v", a, b, n)
 
 
+# ---- products of quantised language models --------------------------------------------
+def _opt(x) -> int:
+    """Address of an operand that may be left out (None or 0)."""
+    return 0 if x is None else addr(x)
+
+
+def gemv_w4_i8(w, scale, x, y, tokens, rows, cols, group, shift):
+    """y[t, r] = (sum_g scale[r, g] * sum_{k in g} w[r, k] * x[t, k]) >> shift, 4-bit weights, int8 x."""
+    return check(lib().__mind_b200_gemv_w4_i8(addr(w), addr(scale), addr(x), addr(y), tokens, rows, cols, group, shift))
+
+
+def gemv_w4_i16(w, scale, x, y, tokens, rows, cols, group, shift):
+    """The same for int16 x."""
+    return check(lib().__mind_b200_gemv_w4_i16(addr(w), addr(scale), addr(x), addr(y), tokens, rows, cols, group, shift))
+
+
+def gemv_w4_q16(w, scale, x, y, tokens, rows, cols, group, shift):
+    """The same for Q16.16 x."""
+    return check(lib().__mind_b200_gemv_w4_q16(addr(w), addr(scale), addr(x), addr(y), tokens, rows, cols, group, shift))
+
+
+def _gemv_w4_grouped(name, w, scale, x, rows_of, offsets, y, m, rows, cols, group, shift, experts, x_rows):
+    return check(getattr(lib(), name)(addr(w), addr(scale), addr(x), _opt(rows_of), addr(offsets), addr(y), m, rows,
+                                      cols, group, shift, experts, x_rows))
+
+
+def gemv_w4_grouped_i8(w, scale, x, rows_of, offsets, y, m, rows, cols, group, shift, experts, x_rows):
+    """``gemv_w4_i8`` with one matrix per expert: rows [offsets[e], offsets[e+1]) of y meet matrix e, and
+    row p of y reads row rows_of[p] of x (None: row p).  ``expert_plan`` makes rows_of and offsets."""
+    return _gemv_w4_grouped("__mind_b200_gemv_w4_grouped_i8", w, scale, x, rows_of, offsets, y, m, rows, cols, group,
+                            shift, experts, x_rows)
+
+
+def gemv_w4_grouped_i16(w, scale, x, rows_of, offsets, y, m, rows, cols, group, shift, experts, x_rows):
+    return _gemv_w4_grouped("__mind_b200_gemv_w4_grouped_i16", w, scale, x, rows_of, offsets, y, m, rows, cols, group,
+                            shift, experts, x_rows)
+
+
+def gemv_w4_grouped_q16(w, scale, x, rows_of, offsets, y, m, rows, cols, group, shift, experts, x_rows):
+    return _gemv_w4_grouped("__mind_b200_gemv_w4_grouped_q16", w, scale, x, rows_of, offsets, y, m, rows, cols, group,
+                            shift, experts, x_rows)
+
+
+def _matmul_grouped(name, a, rows, b, offsets, scale, c, m, k, n, experts, a_rows, shift):
+    return check(getattr(lib(), name)(addr(a), _opt(rows), addr(b), addr(offsets), _opt(scale), addr(c), m, k, n,
+                                      experts, a_rows, shift))
+
+
+def matmul_grouped_i8(a, rows, b, offsets, scale, c, m, k, n, experts, a_rows, shift=0):
+    """int8 products grouped by expert: rows [offsets[e], offsets[e+1]) of c are a[rows[p]] . b[e] (b: experts x
+    k x n; rows None: row p of a), times scale[e, n] >> shift where a scale is given."""
+    return _matmul_grouped("__mind_b200_matmul_grouped_i8", a, rows, b, offsets, scale, c, m, k, n, experts, a_rows, shift)
+
+
+def matmul_grouped_i8_bt(a, rows, bt, offsets, scale, c, m, k, n, experts, a_rows, shift=0):
+    """``matmul_grouped_i8`` with the weights stored transposed (experts x n x k)."""
+    return _matmul_grouped("__mind_b200_matmul_grouped_i8_bt", a, rows, bt, offsets, scale, c, m, k, n, experts, a_rows,
+                           shift)
+
+
+def expert_plan(ids, offsets, rows, place, count, experts, per):
+    """Groups `count` expert ids (`per` of every token) stably by expert: offsets[experts + 1], the token
+    rows[p] of every grouped slot p, and place[i], the slot of id i (-1 where it names no expert)."""
+    return check(lib().__mind_b200_expert_plan(addr(ids), addr(offsets), addr(rows), addr(place), count, experts, per))
+
+
 STATIC_SCRATCH_BYTES = 8 * 1024 * 1024
 
 

@@ -17,6 +17,7 @@ struct Operand {
     void* user = nullptr;
     size_t bytes = 0;
     bool output = false;
+    bool keep = false;    // an output the kernels may leave parts of untouched: uploaded first
     bool host = false;
     bool staged = false;  // pageable and large: moved by the staging threads
     void* dev = nullptr;
@@ -29,12 +30,13 @@ class Call {
 public:
     explicit Call(DeviceCtx* ctx) : ctx_(ctx) {}
 
-    int add(const void* p, size_t bytes, bool output) {
+    int add(const void* p, size_t bytes, bool output, bool keep = false) {
         Operand& o = store_[n_];
         o = Operand();
         o.user = const_cast<void*>(p);
         o.bytes = bytes;
         o.output = output;
+        o.keep = keep;
         return n_++;
     }
 
@@ -73,7 +75,7 @@ public:
             // a large pageable operand goes through the staging threads' pinned slots (several
             // cores copy, the DMAs overlap them) instead of the driver's one-thread staging
             o.staged = o.bytes >= STAGED_MIN_BYTES && host_pointer_is_pageable(o.user) && stager_start();
-            if (o.output) continue;
+            if (o.output && !o.keep) continue;
             if (o.staged) {
                 const size_t row = (size_t)1 << 20, rows = o.bytes / row, rest = o.bytes - rows * row;
                 StageGroup body, tail;
@@ -131,14 +133,15 @@ public:
     static int64_t check_err_word(DeviceCtx* ctx) { return ::mb200::check_err_word(ctx); }
 
 private:
-    // at most four operands per call; iterated as a range
+    // at most MAX_OPERANDS operands per call; iterated as a range
     struct Range {
         Operand *b, *e;
         Operand* begin() const { return b; }
         Operand* end() const { return e; }
     };
+    static constexpr int MAX_OPERANDS = 6;
     DeviceCtx* ctx_;
-    Operand store_[4];
+    Operand store_[MAX_OPERANDS];
     int n_ = 0;
     bool any_host_ = false;
     StageStatus status_;
@@ -778,12 +781,187 @@ int64_t dot(int kind, int64_t a, int64_t b, int64_t len) {
     return (int64_t)result;
 }
 
+// ------------------------------------------- products of quantised language models
+constexpr int64_t MAX_DIM = 0x7fffffff;
+constexpr int64_t MAX_EXPERTS = 4096;  // expert_plan keeps a histogram per warp in shared memory
+
+int64_t check_experts(int64_t experts) {
+    if (experts < 0) return fail(MIND_B200_ERR_INVALID, "negative number of experts");
+    if (experts > MAX_EXPERTS)
+        return fail(MIND_B200_ERR_TOO_LARGE, "%lld experts; at most %lld are supported", (long long)experts, (long long)MAX_EXPERTS);
+    return 0;
+}
+
+// An operand of a * b * c elements: every size within 31 bits, the whole within 62.
+int64_t check_extent(int64_t a, int64_t b, int64_t c) {
+    if (a > MAX_DIM || b > MAX_DIM || c > MAX_DIM) return fail(MIND_B200_ERR_TOO_LARGE, "dimension above 2^31-1");
+    if ((double)a * (double)b * (double)c > 4.6e18) return fail(MIND_B200_ERR_TOO_LARGE, "operand above 2^62 elements");
+    return 0;
+}
+
+// Offsets in host memory can be looked at: they must be a running sum within [0, m].  (Those in
+// device memory are bounded by the kernels.)
+int64_t check_host_offsets(const int32_t* offsets, int64_t experts, int64_t m) {
+    cudaPointerAttributes at;
+    if (cudaPointerGetAttributes(&at, offsets) != cudaSuccess)
+        cudaGetLastError();  // memory CUDA does not know, or no device at all: an ordinary host address
+    else if (at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged)
+        return 0;
+    int64_t before = 0;
+    for (int64_t e = 0; e <= experts; ++e) {
+        if (offsets[e] < before || offsets[e] > m)
+            return fail(MIND_B200_ERR_INVALID, "offsets[%lld] = %d is not a running sum within [0, %lld]", (long long)e,
+                        offsets[e], (long long)m);
+        before = offsets[e];
+    }
+    return 0;
+}
+
+// kind: 0 = int8, 1 = int16, 2 = Q16.16 activations.  offsets = 0: one matrix, x has a row per output row.
+int64_t gemv_w4(int kind, int64_t w, int64_t scale, int64_t x, int64_t rows_of, int64_t offsets, int64_t y, int64_t m,
+                int64_t rows, int64_t cols, int64_t group, int64_t shift, int64_t experts, int64_t x_rows) {
+    clear_error();
+    if (m < 0 || rows < 0 || cols < 0 || x_rows < 0) return fail(MIND_B200_ERR_INVALID, "negative dimension");
+    MB200_TRY(check_experts(experts));
+    if (group <= 0 || group % 32) return fail(MIND_B200_ERR_INVALID, "group must be a positive multiple of 32");
+    if (shift < 0 || shift > 62) return fail(MIND_B200_ERR_INVALID, "shift must be 0..62");
+    if (!rows_of && x_rows != m) return fail(MIND_B200_ERR_INVALID, "without row indices x must have one row per output row");
+    if (m == 0 || rows == 0 || experts == 0) return 0;
+    const int es = kind == 0 ? 1 : (kind == 1 ? 2 : 4);
+    const int64_t pitch = (cols + 1) / 2, groups = (cols + group - 1) / group;
+    MB200_TRY(check_extent(experts, rows, cols));
+    MB200_TRY(check_extent(m, rows, 4));
+    MB200_TRY(check_extent(x_rows, cols, es));
+    if (!y || (cols > 0 && (!w || !scale || (x_rows > 0 && !x)))) return fail(MIND_B200_ERR_INVALID, "null operand");
+    if ((x & (es - 1)) || (scale & 1) || ((y | rows_of | offsets) & 3)) return fail(MIND_B200_ERR_INVALID, "misaligned operand");
+    if (offsets) MB200_TRY(check_host_offsets((const int32_t*)offsets, experts, m));
+    DeviceCtx* ctx = current_ctx();
+    if (!ctx) return MIND_B200_ERR_NO_DEVICE;
+    DevLock lock(ctx->mu);
+    Call call(ctx);
+    const int iw = call.add((void*)w, (size_t)experts * rows * pitch, false);
+    const int is = call.add((void*)scale, (size_t)experts * rows * groups * 2, false);
+    const int ix = call.add((void*)x, (size_t)x_rows * cols * es, false);
+    const int ir = call.add((void*)rows_of, rows_of ? (size_t)m * 4 : 0, false);
+    const int io = call.add((void*)offsets, offsets ? (size_t)(experts + 1) * 4 : 0, false);
+    const int iy = call.add((void*)y, (size_t)m * rows * 4, true, offsets != 0);
+    MB200_TRY(call.begin());
+    W4Args a;
+    a.w = call.dev<int8_t>(iw);
+    a.scale = call.dev<int16_t>(is);
+    a.x = call.dev<void>(ix);
+    a.rows_of = call.dev<int32_t>(ir);
+    a.offsets = call.dev<int32_t>(io);
+    a.y = call.dev<int32_t>(iy);
+    a.m = m;
+    a.rows = rows;
+    a.cols = cols;
+    a.group = group;
+    a.experts = experts;
+    a.x_rows = x_rows;
+    a.shift = (int)shift;
+    a.kind = kind;
+    MB200_TRY(launch_gemv_w4(ctx, a));
+    return call.end(true);
+}
+
+int64_t gemv_w4_one(int kind, int64_t w, int64_t scale, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols,
+                    int64_t group, int64_t shift) {
+    return gemv_w4(kind, w, scale, x, 0, 0, y, tokens, rows, cols, group, shift, 1, tokens);
+}
+
+int64_t gemv_w4_grouped(int kind, int64_t w, int64_t scale, int64_t x, int64_t rows_of, int64_t offsets, int64_t y, int64_t m,
+                        int64_t rows, int64_t cols, int64_t group, int64_t shift, int64_t experts, int64_t x_rows) {
+    if (!offsets && m > 0 && experts > 0) {
+        clear_error();
+        return fail(MIND_B200_ERR_INVALID, "null offsets");
+    }
+    return gemv_w4(kind, w, scale, x, rows_of, offsets, y, m, rows, cols, group, shift, experts, x_rows);
+}
+
+int64_t gemm_grouped_i8(bool bt, int64_t a, int64_t rows, int64_t b, int64_t offsets, int64_t scale, int64_t c, int64_t m,
+                        int64_t k, int64_t n, int64_t experts, int64_t a_rows, int64_t shift) {
+    clear_error();
+    MB200_TRY(check_dims(m, k, n));
+    if (a_rows < 0) return fail(MIND_B200_ERR_INVALID, "negative dimension");
+    MB200_TRY(check_experts(experts));
+    if (shift < 0 || shift > 62) return fail(MIND_B200_ERR_INVALID, "shift must be 0..62");
+    if (!rows && a_rows != m) return fail(MIND_B200_ERR_INVALID, "without row indices a must have one row per output row");
+    if (m == 0 || n == 0 || experts == 0) return 0;
+    MB200_TRY(check_extent(experts, k, n));
+    MB200_TRY(check_extent(m, n, 4));
+    MB200_TRY(check_extent(a_rows, k, 1));
+    if (!c || !offsets || (k > 0 && (!b || (a_rows > 0 && !a)))) return fail(MIND_B200_ERR_INVALID, "null operand");
+    if ((rows | offsets | scale | c) & 3) return fail(MIND_B200_ERR_INVALID, "int32 operand is not 4-byte aligned");
+    MB200_TRY(check_host_offsets((const int32_t*)offsets, experts, m));
+    DeviceCtx* ctx = current_ctx();
+    if (!ctx) return MIND_B200_ERR_NO_DEVICE;
+    DevLock lock(ctx->mu);
+    Call call(ctx);
+    const int ia = call.add((void*)a, (size_t)a_rows * k, false);
+    const int ir = call.add((void*)rows, rows ? (size_t)m * 4 : 0, false);
+    const int ib = call.add((void*)b, (size_t)experts * k * n, false);
+    const int io = call.add((void*)offsets, (size_t)(experts + 1) * 4, false);
+    const int is = call.add((void*)scale, scale ? (size_t)experts * n * 4 : 0, false);
+    const int ic = call.add((void*)c, (size_t)m * n * 4, true, true);
+    MB200_TRY(call.begin());
+    GroupedArgs g;
+    g.a = call.dev<int8_t>(ia);
+    g.rows = call.dev<int32_t>(ir);
+    g.b = call.dev<int8_t>(ib);
+    g.offsets = call.dev<int32_t>(io);
+    g.scale = call.dev<int32_t>(is);
+    g.c = call.dev<int32_t>(ic);
+    g.m = m;
+    g.k = k;
+    g.n = n;
+    g.experts = experts;
+    g.a_rows = a_rows;
+    g.shift = (int)shift;
+    g.bt = bt ? 1 : 0;
+    MB200_TRY(launch_gemm_grouped_i8(ctx, g));
+    return call.end(true);
+}
+
+int64_t expert_plan(int64_t ids, int64_t offsets, int64_t rows, int64_t place, int64_t count, int64_t experts, int64_t per) {
+    clear_error();
+    if (count < 0) return fail(MIND_B200_ERR_INVALID, "negative count");
+    MB200_TRY(check_experts(experts));
+    if (experts == 0) return fail(MIND_B200_ERR_INVALID, "no experts");
+    if (per <= 0) return fail(MIND_B200_ERR_INVALID, "per must be positive");
+    if (count > MAX_DIM) return fail(MIND_B200_ERR_TOO_LARGE, "count above 2^31-1");
+    if (!offsets || (count > 0 && (!ids || !rows || !place))) return fail(MIND_B200_ERR_INVALID, "null operand");
+    if ((ids | offsets | rows | place) & 3) return fail(MIND_B200_ERR_INVALID, "int32 operand is not 4-byte aligned");
+    DeviceCtx* ctx = current_ctx();
+    if (!ctx) return MIND_B200_ERR_NO_DEVICE;
+    DevLock lock(ctx->mu);
+    Call call(ctx);
+    const int ii = call.add((void*)ids, (size_t)count * 4, false);
+    const int io = call.add((void*)offsets, (size_t)(experts + 1) * 4, true);
+    const int ir = call.add((void*)rows, (size_t)count * 4, true, true);
+    const int ip = call.add((void*)place, (size_t)count * 4, true);
+    MB200_TRY(call.begin());
+    MB200_TRY(launch_expert_plan(ctx, call.dev<int32_t>(ii), call.dev<int32_t>(io), call.dev<int32_t>(ir),
+                                 call.dev<int32_t>(ip), count, experts, per));
+    return call.end();
+}
+
 }  // namespace
 }  // namespace mb200
 
 using namespace mb200;
 
 extern "C" {
+
+int64_t __mind_b200_gemv_w4_i8(int64_t w, int64_t s, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols, int64_t group, int64_t shift) { return gemv_w4_one(0, w, s, x, y, tokens, rows, cols, group, shift); }
+int64_t __mind_b200_gemv_w4_i16(int64_t w, int64_t s, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols, int64_t group, int64_t shift) { return gemv_w4_one(1, w, s, x, y, tokens, rows, cols, group, shift); }
+int64_t __mind_b200_gemv_w4_q16(int64_t w, int64_t s, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols, int64_t group, int64_t shift) { return gemv_w4_one(2, w, s, x, y, tokens, rows, cols, group, shift); }
+int64_t __mind_b200_gemv_w4_grouped_i8(int64_t w, int64_t s, int64_t x, int64_t r, int64_t o, int64_t y, int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t shift, int64_t experts, int64_t x_rows) { return gemv_w4_grouped(0, w, s, x, r, o, y, m, rows, cols, group, shift, experts, x_rows); }
+int64_t __mind_b200_gemv_w4_grouped_i16(int64_t w, int64_t s, int64_t x, int64_t r, int64_t o, int64_t y, int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t shift, int64_t experts, int64_t x_rows) { return gemv_w4_grouped(1, w, s, x, r, o, y, m, rows, cols, group, shift, experts, x_rows); }
+int64_t __mind_b200_gemv_w4_grouped_q16(int64_t w, int64_t s, int64_t x, int64_t r, int64_t o, int64_t y, int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t shift, int64_t experts, int64_t x_rows) { return gemv_w4_grouped(2, w, s, x, r, o, y, m, rows, cols, group, shift, experts, x_rows); }
+int64_t __mind_b200_matmul_grouped_i8(int64_t a, int64_t r, int64_t b, int64_t o, int64_t s, int64_t c, int64_t m, int64_t k, int64_t n, int64_t experts, int64_t a_rows, int64_t shift) { return gemm_grouped_i8(false, a, r, b, o, s, c, m, k, n, experts, a_rows, shift); }
+int64_t __mind_b200_matmul_grouped_i8_bt(int64_t a, int64_t r, int64_t b, int64_t o, int64_t s, int64_t c, int64_t m, int64_t k, int64_t n, int64_t experts, int64_t a_rows, int64_t shift) { return gemm_grouped_i8(true, a, r, b, o, s, c, m, k, n, experts, a_rows, shift); }
+int64_t __mind_b200_expert_plan(int64_t ids, int64_t offsets, int64_t rows, int64_t place, int64_t count, int64_t experts, int64_t per) { return expert_plan(ids, offsets, rows, place, count, experts, per); }
 
 int64_t __mind_blas_matmul_mm_i8_v(int64_t a, int64_t b, int64_t c, int64_t m, int64_t k, int64_t n) { return gemm_i8(a, b, c, m, k, n); }
 int64_t __mind_blas_matmul_mm_i8_mt_v(int64_t a, int64_t b, int64_t c, int64_t m, int64_t k, int64_t n) { return gemm_i8(a, b, c, m, k, n); }

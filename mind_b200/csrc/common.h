@@ -288,6 +288,34 @@ int64_t launch_gemv_i16(DeviceCtx* ctx, const int16_t* w, const int16_t* x, int3
                         int64_t rows, int64_t cols);
 int64_t launch_dist_l1_q16(DeviceCtx* ctx, const int32_t* a, const int32_t* b, int32_t* out,
                            int64_t len);
+// ---- products of quantised language models (gemv_w4.cu, gemm_grouped.cu, plan.cu) ----
+// Rows [offsets[e], offsets[e + 1]) of the output belong to expert e (offsets null: one matrix, all
+// rows).  Offsets live on the device, where only the kernels see them: they take each bound no lower
+// than the one before and no higher than m, so that wrong offsets never address outside the output.
+struct W4Args {
+    const int8_t* w;        // experts x rows x ceil(cols / 2)
+    const int16_t* scale;   // experts x rows x ceil(cols / group)
+    const void* x;          // x_rows x cols, of `kind`: 0 = int8, 1 = int16, 2 = Q16.16
+    const int32_t* rows_of; // row of x of every output row, or null: the same row
+    const int32_t* offsets;
+    int32_t* y;             // m x rows
+    int64_t m, rows, cols, group, experts, x_rows;
+    int shift, kind;
+};
+int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a);
+struct GroupedArgs {
+    const int8_t* a;        // a_rows x k
+    const int32_t* rows;    // row of a of every output row, or null: the same row
+    const int8_t* b;        // experts x k x n, or (bt) experts x n x k
+    const int32_t* offsets;
+    const int32_t* scale;   // experts x n, or null
+    int32_t* c;             // m x n
+    int64_t m, k, n, experts, a_rows;
+    int shift, bt;
+};
+int64_t launch_gemm_grouped_i8(DeviceCtx* ctx, const GroupedArgs& g);
+int64_t launch_expert_plan(DeviceCtx* ctx, const int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* place,
+                           int64_t count, int64_t experts, int64_t per);
 int64_t launch_lcg_fill(DeviceCtx* ctx, void* dst, int64_t n, int kind, uint64_t seed,
                         uint64_t offset, int shift);
 int64_t measure_fp64_fma_peak(DeviceCtx* ctx, double* fma_per_s, double* sm_mhz);

@@ -1,0 +1,553 @@
+"""Products of quantised language models: 4-bit matrix-vector products, int8 products grouped by
+expert, and the plan that groups slots by expert.  Everything is integer arithmetic with one right
+answer, so every comparison is for equality with numpy's int64 (tolerance zero: each output is the
+exact sum, or its low 64 bits, shifted and truncated once)."""
+import threading
+
+import numpy as np
+import pytest
+
+import mind_b200
+from mind_b200 import blas
+
+I32 = np.int32
+CANARY = 0x5A5A5A5A
+
+
+# ------------------------------------------------------------------- plain implementations
+def low32(v):
+    return (v.astype(np.int64) & 0xFFFFFFFF).astype(np.uint32).view(np.int32)
+
+
+def unpack4(w, cols):
+    """(…, pitch) int8 -> (…, cols) int64, even column in the low half."""
+    b = w.astype(np.int64) & 255
+    d = np.stack([b & 15, b >> 4], axis=-1).reshape(*w.shape[:-1], -1)
+    return ((d ^ 8) - 8)[..., :cols]
+
+
+def ref_w4(w, scale, x, cols, group, shift):
+    """int64 throughout; numpy's int64 wraps mod 2^64, as the definition does."""
+    d = unpack4(w, cols)
+    total = np.zeros((x.shape[0], w.shape[0]), np.int64)
+    with np.errstate(over="ignore"):
+        for g in range(scale.shape[1]):
+            k0, k1 = g * group, min(cols, (g + 1) * group)
+            total += (x[:, k0:k1].astype(np.int64) @ d[:, k0:k1].T) * scale[:, g].astype(np.int64)
+    return low32(total >> shift)
+
+
+def gather(x, rows_of, p, width):
+    out = np.zeros((len(p), width), np.int64)
+    for j, q in enumerate(p):
+        r = q if rows_of is None else rows_of[q]
+        if 0 <= r < x.shape[0]:
+            out[j] = x[r]
+    return out
+
+
+def ref_w4_grouped(w, scale, x, rows_of, offsets, y, cols, group, shift):
+    y = y.copy()
+    for e in range(w.shape[0]):
+        p = np.arange(offsets[e], offsets[e + 1])
+        if len(p):
+            y[p] = ref_w4(w[e], scale[e], gather(x, rows_of, p, cols), cols, group, shift)
+    return y
+
+
+def ref_grouped(a, rows, b, offsets, scale, c, shift, bt):
+    c = c.copy()
+    for e in range(b.shape[0]):
+        p = np.arange(offsets[e], offsets[e + 1])
+        if not len(p):
+            continue
+        be = b[e].T if bt else b[e]
+        # float64 is exact for these sums (below 2^53) and much faster than int64 @
+        acc = low32((gather(a, rows, p, be.shape[0]).astype(np.float64) @ be.astype(np.float64)).astype(np.int64))
+        c[p] = acc if scale is None else low32((acc.astype(np.int64) * scale[e].astype(np.int64)) >> shift)
+    return c
+
+
+def ref_plan(ids, experts, per, rows):
+    rows, place = rows.copy(), np.full(ids.size, -1, I32)
+    offsets, at = np.zeros(experts + 1, I32), 0
+    for e in range(experts):
+        for i in np.flatnonzero(ids == e):
+            rows[at], place[i], at = i // per, at, at + 1
+        offsets[e + 1] = at
+    return offsets, rows, place
+
+
+def sizes_to_offsets(sizes, start=0):
+    return np.concatenate([[start], start + np.cumsum(sizes)]).astype(I32)
+
+
+def x_of(rng, kind, shape, extreme=False):
+    t = {"i8": np.int8, "i16": np.int16, "q16": np.int32}[kind]
+    i = np.iinfo(t)
+    if extreme:
+        return rng.choice(np.array([i.min, i.min + 1, -1, 0, 1, i.max - 1, i.max], t), shape)
+    return rng.integers(i.min, i.max, shape, dtype=t, endpoint=True)
+
+
+def w4_of(rng, *shape):
+    return rng.integers(-128, 127, shape, dtype=np.int8, endpoint=True)
+
+
+def scale_of(rng, *shape):
+    return rng.integers(-32768, 32767, shape, dtype=np.int16, endpoint=True)
+
+
+# ------------------------------------------------------------------------ refusals (no GPU)
+W, S, X, Y = np.zeros(64, np.int8), np.zeros(8, np.int16), np.zeros(64, I32), np.zeros(64, I32)
+OFF = np.array([0, 1, 2], I32)
+
+
+def refused(code, fn, *args):
+    with pytest.raises(mind_b200.MindB200Error) as e:
+        fn(*args)
+    assert e.value.code == code, str(e.value)
+
+
+@pytest.mark.parametrize("fn", [blas.gemv_w4_i8, blas.gemv_w4_i16, blas.gemv_w4_q16])
+def test_gemv_w4_refuses(fn):
+    bad = lambda *a: refused(mind_b200.ERR_INVALID, fn, *a)  # noqa: E731
+    bad(W, S, X, Y, -1, 1, 32, 32, 0)
+    bad(W, S, X, Y, 1, -1, 32, 32, 0)
+    bad(W, S, X, Y, 1, 1, -1, 32, 0)
+    bad(W, S, X, Y, 1, 1, 32, 0, 0)
+    bad(W, S, X, Y, 1, 1, 32, 48, 0)
+    bad(W, S, X, Y, 1, 1, 32, -32, 0)
+    bad(W, S, X, Y, 1, 1, 32, 32, -1)
+    bad(W, S, X, Y, 1, 1, 32, 32, 63)
+    bad(0, S, X, Y, 1, 1, 32, 32, 0)
+    bad(W, 0, X, Y, 1, 1, 32, 32, 0)
+    bad(W, S, 0, Y, 1, 1, 32, 32, 0)
+    bad(W, S, X, 0, 1, 1, 32, 32, 0)
+    bad(W, S.ctypes.data + 1, X, Y, 1, 1, 32, 32, 0)
+    bad(W, S, X, Y.ctypes.data + 2, 1, 1, 32, 32, 0)
+    if fn is not blas.gemv_w4_i8:
+        bad(W, S, X.ctypes.data + 1, Y, 1, 1, 32, 32, 0)
+    refused(mind_b200.ERR_TOO_LARGE, fn, W, S, X, Y, 1, 1 << 31, 32, 32, 0)
+    refused(mind_b200.ERR_TOO_LARGE, fn, W, S, X, Y, 1, 1, 1 << 31, 32, 0)
+    assert fn(0, 0, 0, 0, 0, 5, 32, 32, 0) == 0  # nothing to do
+    assert fn(0, 0, 0, 0, 5, 0, 32, 32, 0) == 0
+
+
+def test_gemv_w4_grouped_refuses():
+    fn = blas.gemv_w4_grouped_i8
+    bad = lambda *a: refused(mind_b200.ERR_INVALID, fn, *a)  # noqa: E731
+    bad(W, S, X, 0, 0, Y, 2, 1, 32, 32, 0, 2, 2)  # no offsets
+    bad(W, S, X, 0, OFF, Y, 2, 1, 32, 32, 0, 2, 3)  # no row indices, but x has another number of rows
+    bad(W, S, X, 0, OFF, Y, 2, 1, 32, 32, 0, -1, 2)
+    bad(W, S, X, 0, OFF.ctypes.data + 1, Y, 2, 1, 32, 32, 0, 2, 2)
+    bad(W, S, X, 0, np.array([0, 3, 2], I32), Y, 2, 1, 32, 32, 0, 2, 2)
+    bad(W, S, X, 0, np.array([-1, 1, 2], I32), Y, 2, 1, 32, 32, 0, 2, 2)
+    bad(W, S, X, 0, np.array([0, 1, 3], I32), Y, 2, 1, 32, 32, 0, 2, 2)
+    refused(mind_b200.ERR_TOO_LARGE, fn, W, S, X, 0, OFF, Y, 2, 1, 32, 32, 0, 4097, 2)
+
+
+@pytest.mark.parametrize("fn", [blas.matmul_grouped_i8, blas.matmul_grouped_i8_bt])
+def test_matmul_grouped_refuses(fn):
+    bad = lambda *a: refused(mind_b200.ERR_INVALID, fn, *a)  # noqa: E731
+    bad(W, 0, W, OFF, 0, Y, -1, 4, 4, 2, 2)
+    bad(W, 0, W, OFF, 0, Y, 2, -4, 4, 2, 2)
+    bad(W, 0, W, OFF, 0, Y, 2, 4, -4, 2, 2)
+    bad(W, 0, W, OFF, 0, Y, 2, 4, 4, -2, 2)
+    bad(W, 0, W, OFF, 0, Y, 2, 4, 4, 2, 3)  # no row indices, but a has another number of rows
+    bad(W, OFF, W, OFF, 0, Y, 2, 4, 4, 2, -1)
+    bad(W, 0, W, OFF, 0, Y, 2, 4, 4, 2, 2, 63)
+    bad(W, 0, W, OFF, 0, Y, 2, 4, 4, 2, 2, -1)
+    bad(0, 0, W, OFF, 0, Y, 2, 4, 4, 2, 2)
+    bad(W, 0, 0, OFF, 0, Y, 2, 4, 4, 2, 2)
+    bad(W, 0, W, 0, 0, Y, 2, 4, 4, 2, 2)
+    bad(W, 0, W, OFF, 0, 0, 2, 4, 4, 2, 2)
+    bad(W, 0, W, OFF, X.ctypes.data + 2, Y, 2, 4, 4, 2, 2)
+    bad(W, 0, W, OFF, 0, Y.ctypes.data + 1, 2, 4, 4, 2, 2)
+    bad(W, 0, W, np.array([0, 2, 1], I32), 0, Y, 2, 4, 4, 2, 2)
+    bad(W, 0, W, np.array([0, 2, 3], I32), 0, Y, 2, 4, 4, 2, 2)
+    refused(mind_b200.ERR_TOO_LARGE, fn, W, 0, W, OFF, 0, Y, 2, 4, 1 << 31, 2, 2)
+    refused(mind_b200.ERR_TOO_LARGE, fn, W, 0, W, OFF, 0, Y, 2, 4, 4, 4097, 2)
+    assert fn(0, 0, 0, 0, 0, 0, 0, 4, 4, 2, 0) == 0
+    assert fn(0, 0, 0, 0, 0, 0, 2, 4, 0, 2, 2) == 0
+    assert fn(0, 0, 0, 0, 0, 0, 2, 4, 4, 0, 2) == 0
+
+
+def test_expert_plan_refuses():
+    bad = lambda *a: refused(mind_b200.ERR_INVALID, blas.expert_plan, *a)  # noqa: E731
+    bad(X, Y, X, Y, -1, 4, 1)
+    bad(X, Y, X, Y, 4, 0, 1)
+    bad(X, Y, X, Y, 4, -4, 1)
+    bad(X, Y, X, Y, 4, 4, 0)
+    bad(0, Y, X, Y, 4, 4, 1)
+    bad(X, 0, X, Y, 4, 4, 1)
+    bad(X, Y, 0, Y, 4, 4, 1)
+    bad(X, Y, X, 0, 4, 4, 1)
+    bad(X.ctypes.data + 1, Y, X, Y, 4, 4, 1)
+    refused(mind_b200.ERR_TOO_LARGE, blas.expert_plan, X, Y, X, Y, 4, 4097, 1)
+    refused(mind_b200.ERR_TOO_LARGE, blas.expert_plan, X, Y, X, Y, 1 << 31, 4, 1)
+
+
+def test_no_gpu_means_a_clean_refusal():
+    if blas.device_count() > 0:
+        pytest.skip("a B200 is present; the refusal path is for machines without one")
+    refused(mind_b200.ERR_NO_DEVICE, blas.gemv_w4_q16, W, S, X, Y, 1, 1, 32, 32, 0)
+    refused(mind_b200.ERR_NO_DEVICE, blas.matmul_grouped_i8, W, 0, W, OFF, 0, Y, 2, 4, 4, 2, 2)
+    refused(mind_b200.ERR_NO_DEVICE, blas.expert_plan, X, Y, X, Y, 4, 4, 1)
+
+
+# ------------------------------------------------------------------------------- on a GPU
+@pytest.fixture(params=[0, 1], ids=["default", "cross-check"])
+def path(request, gpu):
+    """Both kernel families: the default one and the CUDA-core cross-check."""
+    gpu.set_gemm_path(request.param)
+    yield request.param
+    gpu.set_gemm_path(0)
+
+
+@pytest.fixture
+def torch_gpu(gpu):
+    import torch
+    gpu.set_stream(torch.cuda.current_stream().cuda_stream)
+    yield torch
+    gpu.set_stream(0)
+
+
+def dev(torch, *arrays):
+    return [None if a is None else torch.from_numpy(a).cuda() for a in arrays]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,experts,per", [
+    (0, 3, 1), (1, 1, 1), (7, 4, 1), (64, 8, 8), (33, 33, 3), (1000, 5, 2), (1024, 256, 8), (4097, 160, 6), (65536, 64, 8),
+    (70001, 3, 7), (5000, 4096, 2), (300000, 512, 4)])
+def test_expert_plan(gpu, count, experts, per):
+    rng = np.random.default_rng(count * 31 + experts)
+    for padding in (0.0, 0.3, 1.0):
+        ids = rng.integers(0, experts, count, dtype=I32)
+        bad = rng.random(count) < padding
+        ids[bad] = rng.choice(np.array([-1, -(2 ** 31), experts, 2 ** 31 - 1], I32), int(bad.sum()))
+        rows, place, offsets = (np.full(n + 5, CANARY, I32) for n in (count, count, experts + 1))
+        want = ref_plan(ids, experts, per, rows)
+        gpu.expert_plan(ids, offsets, rows, place, count, experts, per)
+        assert np.array_equal(offsets[:experts + 1], want[0])
+        assert np.array_equal(rows, want[1])  # what lies behind the kept slots is as it was
+        assert np.array_equal(place[:count], want[2])
+        assert np.all(place[count:] == CANARY) and np.all(offsets[experts + 1:] == CANARY)
+
+
+@pytest.mark.gpu
+def test_expert_plan_one_popular_expert(gpu):
+    """Every slot of one expert, and experts in descending order."""
+    for ids in (np.full(20000, 6, I32), np.repeat(np.arange(49, -1, -1), 37).astype(I32)):
+        offsets, rows, place = np.zeros(51, I32), np.zeros(ids.size, I32), np.zeros(ids.size, I32)
+        gpu.expert_plan(ids, offsets, rows, place, ids.size, 50, 1)
+        want = ref_plan(ids, 50, 1, rows)
+        for got, expected in zip((offsets, rows, place), want):
+            assert np.array_equal(got, expected)
+
+
+# Block edges of the kernels: 16 rows, 32 / 256 columns, 8 tokens; odd columns (a half-filled last byte).
+W4_SHAPES = [
+    (1, 1, 1, 32), (1, 1, 32, 32), (1, 16, 256, 64), (2, 17, 255, 128), (3, 33, 257, 32), (8, 48, 512, 256),
+    (9, 15, 96, 96), (5, 100, 1000, 64), (4, 64, 2048, 128), (7, 31, 777, 1024), (16, 40, 1056, 32), (17, 129, 640, 160),
+    (32, 65, 800, 128), (33, 20, 320, 64), (70, 18, 416, 32), (1, 300, 4096, 128), (2, 2500, 1024, 512), (3, 1030, 544, 32),
+    (1, 16, 20000, 128), (8, 24, 9000, 64), (6, 40, 0, 32),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["i8", "i16", "q16"])
+def test_gemv_w4_shapes(gpu, path, kind):
+    fn = getattr(gpu, f"gemv_w4_{kind}")
+    for (t, rows, cols, group) in W4_SHAPES:
+        rng = np.random.default_rng(t * 1000003 + rows * 1009 + cols)
+        groups = -(-cols // group)
+        w, s, x = w4_of(rng, rows, (cols + 1) // 2), scale_of(rng, rows, groups), x_of(rng, kind, (t, cols))
+        for shift in (0, 11, 30):
+            y = np.full(t * rows + 8, CANARY, I32)
+            fn(w, s, x, y, t, rows, cols, group, shift)
+            want = ref_w4(w, s, x, cols, group, shift)
+            assert np.array_equal(y[:t * rows].reshape(t, rows), want), (t, rows, cols, group, shift)
+            assert np.all(y[t * rows:] == CANARY)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["i8", "i16", "q16"])
+def test_gemv_w4_extreme_values(gpu, path, kind):
+    """The ends of every type, all at once and mixed: nothing saturates, every limb carries."""
+    rng = np.random.default_rng(5)
+    i = np.iinfo({"i8": np.int8, "i16": np.int16, "q16": np.int32}[kind])
+    for (t, rows, cols, group) in [(1, 32, 4096, 4096), (8, 16, 1024, 1024), (2, 16, 8192, 32), (3, 50, 333, 64)]:
+        groups = -(-cols // group)
+        cases = [(np.full((rows, (cols + 1) // 2), -120, np.int8), v, m) for v in (i.min, i.max) for m in (-32768, 32767)]
+        cases += [(w4_of(rng, rows, (cols + 1) // 2), None, None)]
+        for w, v, m in cases:
+            x = x_of(rng, kind, (t, cols), extreme=True) if v is None else np.full((t, cols), v, dtype=i.dtype)
+            s = scale_of(rng, rows, groups) if m is None else np.full((rows, groups), m, np.int16)
+            for shift in (0, 20, 62):
+                y = np.empty((t, rows), I32)
+                getattr(gpu, f"gemv_w4_{kind}")(w, s, x, y, t, rows, cols, group, shift)
+                assert np.array_equal(y, ref_w4(w, s, x, cols, group, shift)), (t, rows, cols, shift, v, m)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["i8", "i16", "q16"])
+def test_gemv_w4_odd_bases(torch_gpu, gpu, path, kind):
+    """Device operands whose bases are aligned to their element alone."""
+    torch = torch_gpu
+    rng = np.random.default_rng(9)
+    for (t, rows, cols, group) in [(1, 40, 512, 128), (5, 33, 1024, 32)]:
+        w, s, x = w4_of(rng, rows, cols // 2), scale_of(rng, rows, cols // group), x_of(rng, kind, (t, cols))
+        want = ref_w4(w, s, x, cols, group, 9)
+
+        def shifted(a, by=1):
+            base = torch.zeros(a.size + by, dtype=torch.from_numpy(a).dtype, device="cuda")
+            base[by:] = torch.from_numpy(a.reshape(-1)).cuda()
+            return base[by:]
+
+        y = torch.full((t * rows + 3,), CANARY, dtype=torch.int32, device="cuda")
+        getattr(gpu, f"gemv_w4_{kind}")(shifted(w, 3), shifted(s), shifted(x), y[1:], t, rows, cols, group, 9)
+        got = y.cpu().numpy()
+        assert np.array_equal(got[1:1 + t * rows].reshape(t, rows), want)
+        assert got[0] == CANARY and np.all(got[1 + t * rows:] == CANARY)
+
+
+GROUP_SIZES = [[1], [5, 0, 3], [0, 0, 7, 0], [16, 17, 1, 40], [0], [9, 33, 64, 2, 0, 1]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["i8", "i16", "q16"])
+@pytest.mark.parametrize("sizes", GROUP_SIZES, ids=str)
+def test_gemv_w4_grouped(gpu, path, kind, sizes):
+    rng = np.random.default_rng(len(sizes) * 7 + sum(sizes))
+    fn = getattr(gpu, f"gemv_w4_grouped_{kind}")
+    for (rows, cols, group) in [(35, 320, 32), (64, 1024, 128), (19, 201, 64)]:
+        experts, groups = len(sizes), -(-cols // group)
+        offsets = sizes_to_offsets(sizes, start=2)  # two rows before the first group, three behind the last
+        m, x_rows = int(offsets[-1]) + 3, 11
+        w, s = w4_of(rng, experts, rows, (cols + 1) // 2), scale_of(rng, experts, rows, groups)
+        x = x_of(rng, kind, (x_rows, cols))
+        rows_of = rng.integers(0, x_rows, m).astype(I32)
+        rows_of[rng.random(m) < 0.1] = rng.choice([-1, x_rows, 2 ** 31 - 1])  # such a row counts as zeros
+        y0 = rng.integers(-9, 9, (m, rows)).astype(I32)
+        y = y0.copy()
+        fn(w, s, x, rows_of, offsets, y, m, rows, cols, group, 7, experts, x_rows)
+        assert np.array_equal(y, ref_w4_grouped(w, s, x, rows_of, offsets, y0, cols, group, 7)), (rows, cols)
+        xm, y = x_of(rng, kind, (m, cols)), y0.copy()
+        fn(w, s, xm, None, offsets, y, m, rows, cols, group, 7, experts, m)
+        assert np.array_equal(y, ref_w4_grouped(w, s, xm, None, offsets, y0, cols, group, 7)), (rows, cols)
+
+
+# Tile edges of the grouped kernels: 32 / 128 / 256 rows, 64 / 128 / 256 columns, 128 of K, 16-byte pitches.
+GROUPED_SHAPES = [
+    ([1], 16, 16), ([3, 0, 130], 128, 64), ([129, 257, 1], 144, 272), ([0, 0, 31], 1, 1), ([40, 41], 129, 130),
+    ([300, 5, 0, 64], 256, 256), ([7] * 20, 400, 48), ([500, 20], 96, 528), ([2, 2, 2], 33, 20), ([256, 128], 1040, 128),
+    ([12, 0, 9], 0, 40),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bt", [False, True], ids=["kn", "nk"])
+@pytest.mark.parametrize("sizes,k,n", GROUPED_SHAPES, ids=str)
+def test_matmul_grouped_shapes(gpu, path, bt, sizes, k, n):
+    rng = np.random.default_rng(sum(sizes) + k * 7 + n)
+    experts = len(sizes)
+    fn = gpu.matmul_grouped_i8_bt if bt else gpu.matmul_grouped_i8
+    offsets = sizes_to_offsets(sizes, start=3)
+    m, a_rows = int(offsets[-1]) + 2, 50
+    b = rng.integers(-128, 127, (experts, n, k) if bt else (experts, k, n), dtype=np.int8, endpoint=True)
+    scale = rng.integers(-(2 ** 31), 2 ** 31 - 1, (experts, n), dtype=I32, endpoint=True)
+    c0 = rng.integers(-9, 9, (m, n)).astype(I32)
+    rows = rng.integers(0, a_rows, m).astype(I32)
+    rows[rng.random(m) < 0.1] = rng.choice([-1, a_rows, 2 ** 31 - 1])
+    for ri in (rows, None):
+        a = rng.integers(-128, 127, (a_rows if ri is not None else m, k), dtype=np.int8, endpoint=True)
+        for sc, shift in ((None, 0), (scale, 0), (scale, 31), (scale, 62)):
+            c = c0.copy()
+            fn(a, ri, b, offsets, sc, c, m, k, n, experts, a.shape[0], shift)
+            assert np.array_equal(c, ref_grouped(a, ri, b, offsets, sc, c0, shift, bt)), (ri is not None, shift)
+
+
+@pytest.mark.gpu
+def test_matmul_grouped_wraps(gpu, path):
+    """Sums past 2^31 wrap (K * 2^14 with K = 2^17 + 256), with and without a scale."""
+    k = (1 << 17) + 256
+    a, b = np.full((3, k), -128, np.int8), np.full((2, k, 16), -128, np.int8)
+    offsets, scale = np.array([0, 1, 3], I32), np.full((2, 16), -3, I32)
+    want = low32(np.full((3, 16), k << 14, np.int64))
+    for sc in (None, scale):
+        c = np.zeros((3, 16), I32)
+        gpu.matmul_grouped_i8(a, None, b, offsets, sc, c, 3, k, 16, 2, 3, 1)
+        assert np.array_equal(c, want if sc is None else low32((want.astype(np.int64) * -3) >> 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bt", [False, True], ids=["kn", "nk"])
+def test_matmul_grouped_device_operands(torch_gpu, gpu, path, bt):
+    """Device operands, aligned and not, on sizes where whole and partial tiles meet."""
+    torch = torch_gpu
+    rng = np.random.default_rng(21)
+    fn = gpu.matmul_grouped_i8_bt if bt else gpu.matmul_grouped_i8
+    sizes, k, n = [700, 0, 33, 1, 260], 384, 320
+    offsets = sizes_to_offsets(sizes)
+    m = int(offsets[-1])
+    a = rng.integers(-128, 127, (m, k), dtype=np.int8, endpoint=True)
+    b = rng.integers(-128, 127, (5, n, k) if bt else (5, k, n), dtype=np.int8, endpoint=True)
+    want = ref_grouped(a, None, b, offsets, None, np.zeros((m, n), I32), 0, bt)
+    for by_a, by_b, by_c in ((0, 0, 0), (1, 0, 0), (0, 3, 0), (0, 0, 1), (5, 16, 2)):
+        da, db = torch.zeros(a.size + by_a, dtype=torch.int8, device="cuda"), torch.zeros(b.size + by_b, dtype=torch.int8, device="cuda")
+        da[by_a:], db[by_b:] = torch.from_numpy(a.reshape(-1)).cuda(), torch.from_numpy(b.reshape(-1)).cuda()
+        c = torch.full((m * n + by_c + 4,), CANARY, dtype=torch.int32, device="cuda")
+        fn(da[by_a:], None, db[by_b:], torch.from_numpy(offsets).cuda(), None, c[by_c:], m, k, n, 5, m)
+        got = c.cpu().numpy()
+        assert np.array_equal(got[by_c:by_c + m * n].reshape(m, n), want), (by_a, by_b, by_c)
+        assert np.all(got[:by_c] == CANARY) and np.all(got[by_c + m * n:] == CANARY)
+
+
+@pytest.mark.gpu
+def test_wrong_device_offsets_stay_inside(torch_gpu, gpu, path):
+    """Offsets in device memory cannot be refused; the kernels take each bound no lower than the one before
+    and no higher than m, so nothing outside the output is written."""
+    torch = torch_gpu
+    rng = np.random.default_rng(3)
+    m, k, n, rows = 40, 64, 48, 20
+    a, b = rng.integers(-9, 9, (m, k)).astype(np.int8), rng.integers(-9, 9, (3, k, n)).astype(np.int8)
+    w, s = w4_of(rng, 3, rows, k // 2), scale_of(rng, 3, rows, 2)
+    for off in ([0, 50, 20, 45], [-7, 10, 2 ** 31 - 1, 3], [60, 70, 80, 90], [0, 0, 0, 0], [30, 20, 10, 0]):
+        da, db, dw, ds, do = dev(torch, a, b, w, s, np.array(off, I32))
+        c = torch.full((m * n + 64,), CANARY, dtype=torch.int32, device="cuda")
+        y = torch.full((m * rows + 64,), CANARY, dtype=torch.int32, device="cuda")
+        gpu.matmul_grouped_i8(da, None, db, do, None, c, m, k, n, 3, m)
+        gpu.gemv_w4_grouped_i8(dw, ds, da, None, do, y, m, rows, k, 32, 0, 3, m)
+        gpu.synchronize()
+        assert np.all(c.cpu().numpy()[m * n:] == CANARY) and np.all(y.cpu().numpy()[m * rows:] == CANARY)
+        bounds, before = [], 0
+        for v in off:
+            before = min(max(v, before), m)
+            bounds.append(before)
+        want = ref_grouped(a, None, b, np.array(bounds, I32), None, np.full((m, n), CANARY, I32), 0, False)
+        assert np.array_equal(c.cpu().numpy()[:m * n].reshape(m, n), want), off
+        want = ref_w4_grouped(w, s, a, None, np.array(bounds, I32), np.full((m, rows), CANARY, I32), k, 32, 0)
+        assert np.array_equal(y.cpu().numpy()[:m * rows].reshape(m, rows), want), off
+
+
+def expert_layer(gpu, torch, rng, tokens, per, experts, k, n):
+    """One layer's operands on the device, and what its calls should give."""
+    ids = np.stack([rng.permutation(experts)[:per] for _ in range(tokens)]).astype(I32)
+    ids[tokens - tokens // 5:] = -1  # a padded batch
+    x = rng.integers(-128, 127, (tokens, k), dtype=np.int8, endpoint=True)
+    b = rng.integers(-128, 127, (experts, k, n), dtype=np.int8, endpoint=True)
+    scale = rng.integers(0, 4000, (experts, n)).astype(I32)
+    w, s = w4_of(rng, experts, k, (n + 1) // 2), scale_of(rng, experts, k, -(-n // 64))
+    m = tokens * per
+    offsets, rows, place = ref_plan(ids.reshape(-1), experts, per, np.full(m, CANARY, I32))
+    h = ref_grouped(x, rows, b, offsets, scale, np.full((m, n), CANARY, I32), 6, False)
+    y = ref_w4_grouped(w, s, h, None, offsets, np.full((m, k), CANARY, I32), n, 64, 20)
+    d = dict(zip(("ids", "x", "b", "scale", "w", "s"), dev(torch, ids.reshape(-1), x, b, scale, w, s)))
+    for name, size in (("offsets", experts + 1), ("rows", m), ("place", m), ("h", m * n), ("y", m * k)):
+        d[name] = torch.full((size,), CANARY, dtype=torch.int32, device="cuda")
+
+    def run():
+        gpu.expert_plan(d["ids"], d["offsets"], d["rows"], d["place"], m, experts, per)
+        gpu.matmul_grouped_i8(d["x"], d["rows"], d["b"], d["offsets"], d["scale"], d["h"], m, k, n, experts, tokens, 6)
+        gpu.gemv_w4_grouped_q16(d["w"], d["s"], d["h"], None, d["offsets"], d["y"], m, k, n, 64, 20, experts, m)
+
+    def check():
+        torch.cuda.synchronize()
+        for name, want in (("offsets", offsets), ("rows", rows), ("place", place), ("h", h), ("y", y)):
+            assert np.array_equal(d[name].cpu().numpy(), want.reshape(-1)), name
+
+    return d, run, check
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,per,experts,k,n", [(1, 2, 4, 64, 96), (6, 2, 8, 128, 160), (40, 3, 16, 256, 384),
+                                                    (150, 2, 5, 200, 133)])
+def test_expert_layer(torch_gpu, gpu, path, tokens, per, experts, k, n):
+    """Plan, grouped product, 4-bit product, each fed by the one before, on a padded batch."""
+    _, run, check = expert_layer(gpu, torch_gpu, np.random.default_rng(tokens), tokens, per, experts, k, n)
+    for _ in range(3):
+        run()
+    check()
+
+
+@pytest.mark.gpu
+def test_expert_layer_captured_and_replayed(torch_gpu, gpu):
+    """The layer captured on a side stream and replayed on new tokens: sizes of groups are read on the device."""
+    torch = torch_gpu
+    rng = np.random.default_rng(4)
+    d, run, _ = expert_layer(gpu, torch, rng, 24, 2, 6, 192, 128)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        gpu.set_stream(stream.cuda_stream)
+        run()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            run()
+    for seed in (5, 6):
+        d2, _, _ = expert_layer(gpu, torch, np.random.default_rng(seed), 24, 2, 6, 192, 128)
+        for name in d:
+            d[name].copy_(d2[name])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ids = d["ids"].cpu().numpy()
+        offsets, rows, place = ref_plan(ids, 6, 2, np.full(48, CANARY, I32))
+        h = ref_grouped(d["x"].cpu().numpy(), rows, d["b"].cpu().numpy(), offsets, d["scale"].cpu().numpy(),
+                        np.full((48, 128), CANARY, I32), 6, False)
+        y = ref_w4_grouped(d["w"].cpu().numpy(), d["s"].cpu().numpy(), h, None, offsets, np.full((48, 192), CANARY, I32),
+                           128, 64, 20)
+        for name, want in (("offsets", offsets), ("rows", rows), ("place", place), ("h", h), ("y", y)):
+            assert np.array_equal(d[name].cpu().numpy(), want.reshape(-1)), name
+    gpu.set_stream(0)
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once(torch_gpu, gpu):
+    torch = torch_gpu
+    layers = [expert_layer(gpu, torch, np.random.default_rng(s), 30, 2, 6, 160, 224) for s in (1, 2)]
+    errors = []
+
+    def work(run):
+        try:
+            for _ in range(20):
+                run()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(layer[1],)) for layer in layers]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for layer in layers:
+        layer[2]()
+
+
+@pytest.mark.gpu
+def test_same_bytes_every_time(torch_gpu, gpu):
+    torch = torch_gpu
+    d, run, check = expert_layer(gpu, torch, np.random.default_rng(8), 64, 4, 8, 256, 512)
+    run()
+    check()
+    first = {n: d[n].clone() for n in ("h", "y")}
+    for _ in range(50):
+        for n in first:
+            d[n].fill_(CANARY)
+        run()
+        for n, v in first.items():
+            assert torch.equal(d[n], v)
+
+
+@pytest.mark.gpu
+def test_operands_of_another_device_are_refused(torch_gpu, gpu):
+    torch = torch_gpu
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    y = torch.zeros(16, dtype=torch.int32, device="cuda:1")
+    z = torch.zeros(64, dtype=torch.int8, device="cuda:0")
+    refused(mind_b200.ERR_INVALID, gpu.gemv_w4_i8, z, z, z, y, 1, 1, 32, 32, 0)
