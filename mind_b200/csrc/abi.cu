@@ -830,6 +830,8 @@ int64_t gemv_w4(int kind, int64_t w, int64_t scale, int64_t x, int64_t rows_of, 
     const int es = kind == 0 ? 1 : (kind == 1 ? 2 : 4);
     const int64_t pitch = (cols + 1) / 2, groups = (cols + group - 1) / group;
     MB200_TRY(check_extent(experts, rows, cols));
+    if (m > MAX_DIM - 1024 || rows > MAX_DIM - 1024 || cols > MAX_DIM - 1024)
+        return fail(MIND_B200_ERR_TOO_LARGE, "dimension above 2^31-1025");
     MB200_TRY(check_extent(m, rows, 4));
     MB200_TRY(check_extent(x_rows, cols, es));
     if (!y || (cols > 0 && (!w || !scale || (x_rows > 0 && !x)))) return fail(MIND_B200_ERR_INVALID, "null operand");
@@ -889,6 +891,9 @@ int64_t gemm_grouped_i8(bool bt, int64_t a, int64_t rows, int64_t b, int64_t off
     if (!rows && a_rows != m) return fail(MIND_B200_ERR_INVALID, "without row indices a must have one row per output row");
     if (m == 0 || n == 0 || experts == 0) return 0;
     MB200_TRY(check_extent(experts, k, n));
+    // (tile arithmetic of the kernels: a tile's rows and columns past the end stay within 31 bits)
+    if (m > MAX_DIM - 1024 || n > MAX_DIM - 1024 || k > MAX_DIM - 1024)
+        return fail(MIND_B200_ERR_TOO_LARGE, "dimension above 2^31-1025");
     MB200_TRY(check_extent(m, n, 4));
     MB200_TRY(check_extent(a_rows, k, 1));
     if (!c || !offsets || (k > 0 && (!b || (a_rows > 0 && !a)))) return fail(MIND_B200_ERR_INVALID, "null operand");

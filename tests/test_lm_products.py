@@ -197,10 +197,22 @@ def test_no_gpu_means_a_clean_refusal():
 
 
 # ------------------------------------------------------------------------------- on a GPU
-@pytest.fixture(params=[0, 1], ids=["default", "cross-check"])
+PATHS = {"default": 0, "cross-check": 1}
+GROUPED_PATHS = {**PATHS, "pairs": 2, "single": 3, "small": 10}
+
+
+@pytest.fixture(params=list(PATHS))
 def path(request, gpu):
     """Both kernel families: the default one and the CUDA-core cross-check."""
-    gpu.set_gemm_path(request.param)
+    gpu.set_gemm_path(PATHS[request.param])
+    yield request.param
+    gpu.set_gemm_path(0)
+
+
+@pytest.fixture(params=list(GROUPED_PATHS))
+def grouped_path(request, gpu):
+    """The grouped product's kernels: by shape, cross-check, 256-row tiles on CTA pairs, 128-row, 32-row tiles."""
+    gpu.set_gemm_path(GROUPED_PATHS[request.param])
     yield request.param
     gpu.set_gemm_path(0)
 
@@ -350,7 +362,7 @@ GROUPED_SHAPES = [
 @pytest.mark.gpu
 @pytest.mark.parametrize("bt", [False, True], ids=["kn", "nk"])
 @pytest.mark.parametrize("sizes,k,n", GROUPED_SHAPES, ids=str)
-def test_matmul_grouped_shapes(gpu, path, bt, sizes, k, n):
+def test_matmul_grouped_shapes(gpu, grouped_path, bt, sizes, k, n):
     rng = np.random.default_rng(sum(sizes) + k * 7 + n)
     experts = len(sizes)
     fn = gpu.matmul_grouped_i8_bt if bt else gpu.matmul_grouped_i8
@@ -370,7 +382,7 @@ def test_matmul_grouped_shapes(gpu, path, bt, sizes, k, n):
 
 
 @pytest.mark.gpu
-def test_matmul_grouped_wraps(gpu, path):
+def test_matmul_grouped_wraps(gpu, grouped_path):
     """Sums past 2^31 wrap (K * 2^14 with K = 2^17 + 256), with and without a scale."""
     k = (1 << 17) + 256
     a, b = np.full((3, k), -128, np.int8), np.full((2, k, 16), -128, np.int8)
@@ -384,7 +396,7 @@ def test_matmul_grouped_wraps(gpu, path):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("bt", [False, True], ids=["kn", "nk"])
-def test_matmul_grouped_device_operands(torch_gpu, gpu, path, bt):
+def test_matmul_grouped_device_operands(torch_gpu, gpu, grouped_path, bt):
     """Device operands, aligned and not, on sizes where whole and partial tiles meet."""
     torch = torch_gpu
     rng = np.random.default_rng(21)
@@ -406,7 +418,7 @@ def test_matmul_grouped_device_operands(torch_gpu, gpu, path, bt):
 
 
 @pytest.mark.gpu
-def test_wrong_device_offsets_stay_inside(torch_gpu, gpu, path):
+def test_wrong_device_offsets_stay_inside(torch_gpu, gpu, grouped_path):
     """Offsets in device memory cannot be refused; the kernels take each bound no lower than the one before
     and no higher than m, so nothing outside the output is written."""
     torch = torch_gpu
