@@ -6,8 +6,8 @@
 // B is experts x K x N (N contiguous) or, transposed, experts x N x K.
 //
 // gemm_grouped_tc_kernel, the default, is a persistent warp-specialised tcgen05 kernel:
-//   warp 0     : TMA producer - tiles of A (rows gathered four at a time where `rows` is given) and of
-//                the expert's B into a ring of shared-memory stages of 128 of K;
+//   warp 0     : TMA producer - tiles of A and of the expert's B into a ring of shared-memory stages of
+//                128 of K;
 //   warp 1     : one thread issues tcgen05.mma kind::i8 into two TMEM accumulators in turn;
 //   warps 2..5 : drain an accumulator (each warp 32 rows), scale, store.
 // The groups' bounds are read on the device: every CTA turns the offsets into a table of tiles per
@@ -71,6 +71,83 @@ gemm_grouped_simt_kernel(const GroupedArgs g) {
     }
 }
 
+// ------------------------------------------------------------------ rows made ready
+// dst[i][0 .. pitch) = src[idx ? idx[i] : i][0 .. cols), zeros behind; a row outside [0, src_rows) is
+// zeros.  A warp takes a row, a lane 16 bytes at a time; a source that is not 16-byte aligned is read
+// as the aligned words around the bytes (only words that lie wholly inside src) and shifted together.
+// Bound by memory: cols read, pitch written.
+__global__ void __launch_bounds__(256)
+copy_rows_kernel(const int8_t* __restrict__ src, const int32_t* __restrict__ idx, int8_t* __restrict__ dst, int64_t rows,
+                 int64_t cols, int64_t pitch, int64_t src_rows) {
+    // Everything before this kernel is complete here, and the product behind it may start only now:
+    // it relies on that for all that this kernel does not write.
+    griddep_wait();
+    griddep_launch_dependents();
+    const int lane = threadIdx.x & 31;
+    const int64_t warp = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
+    const int64_t nwarps = ((int64_t)gridDim.x * blockDim.x) >> 5;
+    const int8_t* const end = src + src_rows * cols;
+    for (int64_t i = warp; i < rows; i += nwarps) {
+        const int64_t r = idx ? idx[i] : i;
+        const bool inside = r >= 0 && r < src_rows;
+        const int8_t* const row = src + (inside ? r : 0) * cols;
+        int8_t* const to = dst + i * pitch;
+        const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15);
+#pragma unroll 4
+        for (int64_t c = lane * 16; c < pitch; c += 512) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            const int64_t left = cols - c;  // bytes of the row from here on
+            if (inside && left >= 16 && off == 0) {
+                v = __ldg(reinterpret_cast<const uint4*>(row + c));
+            } else if (inside && left > 0) {
+                const int by = off & 3;
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(row + c - by);  // 4-byte aligned, by bytes early
+                uint32_t x[5];
+#pragma unroll
+                for (int j = 0; j < 5; ++j) {
+                    const int8_t* at = reinterpret_cast<const int8_t*>(w + j);
+                    const int64_t first = 4 * j - by;  // its first byte, counted from c
+                    x[j] = 0;
+                    if (first >= left || first >= 16) continue;
+                    if (at >= src && at + 4 <= end) {
+                        x[j] = __ldg(w + j);
+                    } else {
+                        for (int b = 0; b < 4; ++b)
+                            if (at + b >= src && at + b < end) x[j] |= (uint32_t)(uint8_t)at[b] << (8 * b);
+                    }
+                }
+                uint32_t y[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] = __funnelshift_r(x[j], x[j + 1], 8 * by);
+                    const int64_t keep = left - 4 * j;  // bytes of this word that belong to the row
+                    if (keep < 4) y[j] = keep <= 0 ? 0u : y[j] & ((1u << (8 * keep)) - 1u);
+                }
+                v = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+            *reinterpret_cast<uint4*>(to + c) = v;
+        }
+    }
+}
+
+int64_t launch_copy_rows(DeviceCtx* ctx, const int8_t* src, const int32_t* idx, int8_t* dst, int64_t rows, int64_t cols,
+                         int64_t pitch, int64_t src_rows) {
+    int64_t blocks = (rows + 7) / 8;
+    if (blocks > (int64_t)ctx->sm_count * 8) blocks = (int64_t)ctx->sm_count * 8;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)blocks, 1, 1);
+    lc.blockDim = dim3(256, 1, 1);
+    lc.stream = ctx->stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = at;
+    lc.numAttrs = 1;
+    MB200_CUDA(cudaLaunchKernelEx(&lc, copy_rows_kernel, src, idx, dst, rows, cols, pitch, src_rows));
+    count_launch();
+    return check_launch("copy_rows_kernel");
+}
+
 // ------------------------------------------------------------------ tensor cores
 constexpr int BLOCK_K = 128;  // bytes of K per stage
 constexpr int UMMA_K = 32;
@@ -81,14 +158,14 @@ constexpr int BAR_BYTES = 1024;
 
 struct GtParams {
     const int32_t* offsets;
-    const int32_t* rows;   // null: A's rows are taken as they lie
     const int32_t* scale;
     int32_t* c;
-    int m, k, n, experts, a_rows;
+    int m, k, n, experts;
+    int early;             // the kernel before this one is a copy_rows_kernel that makes A, and B is the caller's
     int n_tiles, stages, patches;  // ring depth and patches per epilogue warp: what the expert table leaves room for
     int group_m, hint_a, hint_b;
     int shift;
-    int tma_store, scale_vec;
+    int tma_store;
     int* err;
 };
 
@@ -164,8 +241,10 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
         tmem_alloc<PAIR>(smem_u32(misc), TMEM_COLS);
         tmem_relinquish<PAIR>();
     }
-    // from here on global memory is read: the kernel before this one must be done
-    griddep_wait();
+    // From here on global memory is read, so the kernel before this one must be done.  Unless that one
+    // is the copy of A's rows (p.early), which lets this one start only when all before it are done:
+    // then nothing but A has to be waited for, and the first tiles of B are fetched beside the copy.
+    if (!p.early) griddep_wait();
     // ---- the table of tiles: bound = running maximum of the offsets within [0, m], cum = running
     // sum of ceil(rows / TILE_M).  Every thread owns a run of experts.
     {
@@ -228,60 +307,51 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
 
     if (warp == 0) {
         // ------------------------------------------------------------ TMA producer
-        // With gathered rows the whole warp works: lane l brings rows 4l .. 4l + 3 of the tile.
-        const bool gather = p.rows != nullptr;
-        if (gather || lane == 0) {
+        if (lane == 0) {
             const uint64_t pol_a = l2_policy(p.hint_a), pol_b = l2_policy(p.hint_b);
+            Tile t;
+            int row0 = 0, col0 = 0;
+            auto start = [&](int item) {
+                t.locate(item, cum, p.n_tiles, p.group_m);
+                row0 = bound[t.e] + t.tm * TILE_M + (int)cta * A_ROWS;
+                col0 = t.tn * BLOCK_N + (int)cta * B_ROWS;
+            };
+            // with a pair, both CTAs' copies complete on the leader's barrier, which alone expects them
+            auto full = [&](uint32_t s) { return PAIR == 2 ? mapa(full0 + 8 * s, 0) : full0 + 8 * s; };
+            auto load_b = [&](uint32_t s, int kx) {
+                const uint32_t db = tiles0 + s * STAGE_BYTES + A_BYTES, bar = full(s);
+                if (leader) mbar_arrive_expect_tx(full0 + 8 * s, PAIR * STAGE_BYTES);
+#pragma unroll
+                for (int j = 0; j < (BMN ? B_ROWS / 128 : 1); ++j) {
+                    const int x = BMN ? col0 + 128 * j : kx, y = BMN ? kx : col0;
+                    if (PAIR == 2) tma_load_3d_pair(db + j * 128 * BLOCK_K, &tm_b, bar, x, y, t.e, pol_b);
+                    else tma_load_3d(db + j * 128 * BLOCK_K, &tm_b, bar, x, y, t.e, pol_b);
+                }
+            };
+            auto load_a = [&](uint32_t s, int kx) {
+                if (PAIR == 2) tma_load_2d_pair(tiles0 + s * STAGE_BYTES, &tm_a, full(s), kx, row0, pol_a);
+                else tma_load_2d(tiles0 + s * STAGE_BYTES, &tm_a, full(s), kx, row0, pol_a);
+            };
+            int early = 0;  // stages whose B was asked for before the rows of A were ready
+            if (p.early) {
+                if (first_item < total) {
+                    start(first_item);
+                    for (; early < stages && early < k_blocks; ++early) load_b(early, early * BLOCK_K);
+                }
+                griddep_wait();
+            }
             uint32_t s = 0, ph = 1;
             bool ok = true;
-            Tile t;
             for (int item = first_item; ok && item < total; item += step) {
-                t.locate(item, cum, p.n_tiles, p.group_m);
-                const int row0 = bound[t.e] + t.tm * TILE_M + (int)cta * A_ROWS;
-                const int col0 = t.tn * BLOCK_N + (int)cta * B_ROWS;
-                int4 idx = make_int4(p.a_rows, p.a_rows, p.a_rows, p.a_rows);  // a row outside A: zeros, no traffic
-                const bool mine = gather && lane * 4 < A_ROWS;
-                if (mine) {
-                    const int hi = bound[t.e + 1], r = row0 + lane * 4;
-                    auto index = [&](int q) {
-                        const int v = q < hi ? p.rows[q] : -1;
-                        return v < 0 || v >= p.a_rows ? p.a_rows : v;
-                    };
-                    idx = make_int4(index(r), index(r + 1), index(r + 2), index(r + 3));
-                }
+                start(item);
                 for (int kb = 0; kb < k_blocks; ++kb) {
-                    // (one lane waits for the warp, so that all leave together when the wait runs out)
-                    if (lane == 0) ok = wait_bounded(empty0 + 8 * s, ph, abort_s, p.err, 1);
-                    if (gather) ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-                    if (!ok) break;
-                    const uint32_t da = tiles0 + s * STAGE_BYTES, db = da + A_BYTES;
-                    const int kx = kb * BLOCK_K;
-                    // with a pair, both CTAs' copies complete on the leader's barrier, which alone expects them
-                    const uint32_t bar = PAIR == 2 ? mapa(full0 + 8 * s, 0) : full0 + 8 * s;
-                    if (lane == 0) {
-                        if (leader) mbar_arrive_expect_tx(full0 + 8 * s, PAIR * STAGE_BYTES);
-                        if (!gather) {
-                            if (PAIR == 2) tma_load_2d_pair(da, &tm_a, bar, kx, row0, pol_a);
-                            else tma_load_2d(da, &tm_a, bar, kx, row0, pol_a);
-                        }
-                        if (BMN) {
-#pragma unroll
-                            for (int j = 0; j < B_ROWS / 128; ++j) {
-                                if (PAIR == 2) tma_load_3d_pair(db + j * 128 * BLOCK_K, &tm_b, bar, col0 + 128 * j, kx, t.e, pol_b);
-                                else tma_load_3d(db + j * 128 * BLOCK_K, &tm_b, bar, col0 + 128 * j, kx, t.e, pol_b);
-                            }
-                        } else {
-                            if (PAIR == 2) tma_load_3d_pair(db, &tm_b, bar, kx, col0, t.e, pol_b);
-                            else tma_load_3d(db, &tm_b, bar, kx, col0, t.e, pol_b);
-                        }
+                    if (!wait_bounded(empty0 + 8 * s, ph, abort_s, p.err, 1)) {
+                        ok = false;
+                        break;
                     }
-                    if (gather) {
-                        __syncwarp();
-                        if (mine) {
-                            if (PAIR == 2) tma_gather4_pair(da + lane * 4 * BLOCK_K, &tm_a, bar, kx, idx, pol_a);
-                            else tma_gather4(da + lane * 4 * BLOCK_K, &tm_a, bar, kx, idx, pol_a);
-                        }
-                    }
+                    if (early > 0) --early;
+                    else load_b(s, kb * BLOCK_K);
+                    load_a(s, kb * BLOCK_K);
                     if (++s == (uint32_t)stages) {
                         s = 0;
                         ph ^= 1u;
@@ -338,11 +408,12 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
             const uint32_t as = tcount % ACC_STAGES, aph = (tcount / ACC_STAGES) & 1u;
             const int row_first = bound[t.e] + t.tm * TILE_M + (int)cta * A_ROWS + q * 32;
             const int valid = q * 32 < A_ROWS ? bound[t.e + 1] - row_first : 0;  // rows of this expert in the block
-            if (!wait_bounded(tfull0 + 8 * as, aph, abort_s, p.err, 4)) break;
-            tc_fence_after();
             const int col_tile = t.tn * BLOCK_N;
             const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + as * BLOCK_N;
             const int32_t* const scale = p.scale ? p.scale + (size_t)t.e * p.n : nullptr;
+            int f_next = scale && col_tile + lane < p.n ? __ldg(scale + col_tile + lane) : 0;
+            if (!wait_bounded(tfull0 + 8 * as, aph, abort_s, p.err, 4)) break;
+            tc_fence_after();
             for (int c0 = 0; c0 < BLOCK_N && valid > 0; c0 += 32) {
                 const int col = col_tile + c0;
                 if (col >= p.n) break;
@@ -350,25 +421,19 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
                 tmem_ld32(t0 + c0, v);
                 tmem_ld_wait();
                 if (scale) {
-                    // the low 32 bits of (acc * scale) >> shift: a funnel shift of the 64-bit product
+                    // lane j holds the scale of column j; the next block's is fetched before it is needed
+                    const int f = f_next;
+                    f_next = col + 32 + lane < p.n ? __ldg(scale + col + 32 + lane) : 0;
+                    if (p.shift < 32) {  // the low 32 bits of the shifted 64-bit product: a funnel shift
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        int4 f;
-                        if (p.scale_vec) {
-                            f = col + j < p.n ? __ldg(reinterpret_cast<const int4*>(scale + col + j)) : make_int4(0, 0, 0, 0);
-                        } else {
-                            f.x = col + j < p.n ? __ldg(scale + col + j) : 0;
-                            f.y = col + j + 1 < p.n ? __ldg(scale + col + j + 1) : 0;
-                            f.z = col + j + 2 < p.n ? __ldg(scale + col + j + 2) : 0;
-                            f.w = col + j + 3 < p.n ? __ldg(scale + col + j + 3) : 0;
+                        for (int j = 0; j < 32; ++j) {
+                            const int64_t prod = (int64_t)(int32_t)v[j] * __shfl_sync(0xffffffffu, f, j);
+                            v[j] = __funnelshift_r((uint32_t)prod, (uint32_t)((uint64_t)prod >> 32), p.shift);
                         }
-                        const int fs[4] = {f.x, f.y, f.z, f.w};
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int64_t prod = (int64_t)(int32_t)v[j + i] * fs[i];
-                            v[j + i] = p.shift < 32 ? __funnelshift_r((uint32_t)prod, (uint32_t)((uint64_t)prod >> 32), p.shift)
-                                                    : (uint32_t)((int32_t)(prod >> 32) >> (p.shift - 32));
-                        }
+                        for (int j = 0; j < 32; ++j)
+                            v[j] = (uint32_t)(__mulhi((int32_t)v[j], __shfl_sync(0xffffffffu, f, j)) >> (p.shift - 32));
                     }
                 }
                 if (valid >= 32 && p.tma_store) {
@@ -482,11 +547,12 @@ int64_t make_tmap_stack(CUtensorMap* tm, const void* base, int64_t cols, int64_t
 
 // a: pitch pa, b: pitch pb (both 16-byte multiples on 16-byte bases).
 template <int A_ROWS, int BLOCK_N, int PAIR, bool BMN>
-int64_t launch_grouped_tc(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a, int64_t pa, const int8_t* b, int64_t pb) {
+int64_t launch_grouped_tc(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a, int64_t pa, const int8_t* b, int64_t pb,
+                          bool early) {
     constexpr int B_ROWS = BLOCK_N / PAIR;
     constexpr int STAGE_BYTES = (A_ROWS + B_ROWS) * BLOCK_K;
     CUtensorMap ta, tb, tc;
-    MB200_TRY(make_tmap_u8(&ta, a, g.k, g.a_rows, pa, g.rows ? 1 : A_ROWS, BLOCK_K));
+    MB200_TRY(make_tmap_u8(&ta, a, g.k, g.m, pa, A_ROWS, BLOCK_K));
     if (BMN) MB200_TRY(make_tmap_stack(&tb, b, g.n, g.k, g.experts, pb, BLOCK_K));
     else MB200_TRY(make_tmap_stack(&tb, b, g.k, g.n, g.experts, pb, B_ROWS));
     GtParams p;
@@ -494,20 +560,18 @@ int64_t launch_grouped_tc(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a,
     tc = ta;
     if (p.tma_store) MB200_TRY(make_tmap_c32(&tc, g.c, g.n, g.m));
     p.offsets = g.offsets;
-    p.rows = g.rows;
     p.scale = g.scale;
     p.c = g.c;
     p.m = (int)g.m;
     p.k = (int)g.k;
     p.n = (int)g.n;
     p.experts = (int)g.experts;
-    p.a_rows = (int)g.a_rows;
+    p.early = early ? 1 : 0;
     p.n_tiles = (int)((g.n + BLOCK_N - 1) / BLOCK_N);
     p.group_m = 8;
     p.hint_a = 1;
     p.hint_b = 0;
     p.shift = g.shift;
-    p.scale_vec = g.scale && g.n % 4 == 0 && reinterpret_cast<uintptr_t>(g.scale) % 16 == 0 ? 1 : 0;
     p.err = ctx->err_word;
     const int64_t most = (g.m / (A_ROWS * PAIR) + g.experts) * p.n_tiles;  // tiles, however the rows are spread
     if (most > 0x7fffffff - 4096) return fail(MIND_B200_ERR_TOO_LARGE, "too many output tiles");
@@ -565,43 +629,49 @@ int64_t launch_grouped_tc(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a,
 }
 
 template <bool BMN>
-int64_t launch_grouped_any(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a, int64_t pa, const int8_t* b, int64_t pb) {
+int64_t launch_grouped_any(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a, int64_t pa, const int8_t* b, int64_t pb,
+                           bool early) {
     // (a kernel may be asked for by name: mind_b200_set_gemm_path 10 / 3 / 2)
     const int pair = tuning().pair_mode.load(), small = tuning().small_tile.load();
     const int64_t avg = g.m / g.experts;
-    if (small == 1) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb);
-    if (pair == 2) return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb);
-    if (pair == 1) return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb);
-    if (avg <= 48) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb);
-    if (avg < 384) return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb);
-    return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb);
+    if (small == 1) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
+    if (pair == 2) return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb, early);
+    if (pair == 1) return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb, early);
+    if (avg <= 48) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
+    if (avg < 384) return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb, early);
+    return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb, early);
 }
 
 }  // namespace
 
 int64_t launch_gemm_grouped_i8(DeviceCtx* ctx, const GroupedArgs& g) {
     if (tuning().gemm_path.load() != 1 && g.k > 0 && g.a_rows > 0) {
-        // TMA reads rows whose pitch and base are multiples of 16 bytes; others are copied to padded rows first
+        // The rows of A as the tiles take them: one under the other in the order of C, on 16-byte pitches and
+        // bases (TMA's rule).  Rows to be gathered, or not aligned, are copied there first; so is an unaligned B.
         const int64_t b_cols = g.bt ? g.k : g.n, b_rows = g.experts * (g.bt ? g.n : g.k);
         const int64_t pa = (int64_t)align_up((size_t)g.k, 16), pb = (int64_t)align_up((size_t)b_cols, 16);
-        const bool a_direct = pa == g.k && reinterpret_cast<uintptr_t>(g.a) % 16 == 0;
+        const bool a_direct = !g.rows && pa == g.k && reinterpret_cast<uintptr_t>(g.a) % 16 == 0;
         const bool b_direct = pb == b_cols && reinterpret_cast<uintptr_t>(g.b) % 16 == 0;
         const int8_t *a = g.a, *b = g.b;
         if (!a_direct || !b_direct) {
-            const size_t sa = a_direct ? 0 : (size_t)g.a_rows * pa, sb = b_direct ? 0 : (size_t)b_rows * pb;
+            const size_t sa = a_direct ? 0 : (size_t)g.m * pa, sb = b_direct ? 0 : (size_t)b_rows * pb;
             MB200_TRY(arena_reserve(ctx, ctx->scratch, align_up(sa, 1024) + align_up(sb, 1024) + 2048));
-            if (!a_direct) {
-                int8_t* to = static_cast<int8_t*>(arena_take(ctx->scratch, sa));
-                MB200_TRY(launch_pad_rows_i8(ctx, g.a, to, g.a_rows, g.k, pa));
-                a = to;
-            }
             if (!b_direct) {
                 int8_t* to = static_cast<int8_t*>(arena_take(ctx->scratch, sb));
-                MB200_TRY(launch_pad_rows_i8(ctx, g.b, to, b_rows, b_cols, pb));
+                MB200_TRY(launch_copy_rows(ctx, g.b, nullptr, to, b_rows, b_cols, pb, b_rows));
                 b = to;
             }
+            if (!a_direct) {
+                int8_t* to = static_cast<int8_t*>(arena_take(ctx->scratch, sa));
+                MB200_TRY(launch_copy_rows(ctx, g.a, g.rows, to, g.m, g.k, pa, g.a_rows));
+                a = to;
+            }
         }
-        return g.bt ? launch_grouped_any<false>(ctx, g, a, pa, b, pb) : launch_grouped_any<true>(ctx, g, a, pa, b, pb);
+        // The copy of A is the last launch before the product, and B (copied before it, or the caller's) is
+        // complete when that copy lets the product start.
+        const bool early = !a_direct;
+        return g.bt ? launch_grouped_any<false>(ctx, g, a, pa, b, pb, early)
+                    : launch_grouped_any<true>(ctx, g, a, pa, b, pb, early);
     }
     int64_t blocks = ((g.n + 31) / 32) * ((g.m + 31) / 32);
     if (blocks > (int64_t)ctx->sm_count * 32) blocks = (int64_t)ctx->sm_count * 32;

@@ -187,25 +187,6 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const void* tmap,
         "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y), "r"(z), "l"(policy)
         : "memory");
 }
-// Four rows y.x .. y.w of a 2-D matrix, from column x, one under the other.  The map's box is one
-// row high; a row outside the matrix arrives as zeros (and counts as delivered bytes).
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const void* tmap, uint32_t bar, int32_t x, int4 y,
-                                            uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint "
-        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w), "l"(policy)
-        : "memory");
-}
-__device__ __forceinline__ void tma_gather4_pair(uint32_t dst, const void* tmap, uint32_t bar, int32_t x, int4 y,
-                                                 uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint "
-        "[%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y.x), "r"(y.y), "r"(y.z), "r"(y.w), "l"(policy)
-        : "memory");
-}
-
 // 2-D tiled store, this CTA's shared memory -> global (rows and columns outside the tensor are
 // clipped by the hardware).  Completion is tracked by the issuing thread's bulk async-group.
 __device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int32_t x, int32_t y) {
