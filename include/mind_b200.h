@@ -121,7 +121,7 @@ int64_t __mind_b200_matmul_mm_i16(int64_t a, int64_t b, int64_t c, int64_t m, in
  *
  * gemv_w4_* multiply 4-bit weights by a few tokens' activations (int8, int16 or Q16.16):
  *   y[t,r] = (i32)( ( sum_g (i64)scale[r,g] * sum_{k in g} W[r,k] * x[t,k] ) >> shift )
- * The sum is taken mod 2^64, shifted (arithmetic, 0..62) and truncated once.  W[r,k] is a signed
+ * The sum is exact mod 2^60, shifted (0..28) and truncated once.  W[r,k] is a signed
  * 4-bit number, two a byte, the even k in the low half, rows of ceil(cols / 2) bytes; group g is
  * columns [g * group, (g + 1) * group), group a positive multiple of 32; scale is
  * int16[rows][ceil(cols / group)].  Scales s are stored as multiples of 2^-f for an f of the

@@ -823,8 +823,8 @@ int64_t gemv_w4(int kind, int64_t w, int64_t scale, int64_t x, int64_t rows_of, 
     clear_error();
     if (m < 0 || rows < 0 || cols < 0 || x_rows < 0) return fail(MIND_B200_ERR_INVALID, "negative dimension");
     MB200_TRY(check_experts(experts));
-    if (group <= 0 || group % 32) return fail(MIND_B200_ERR_INVALID, "group must be a positive multiple of 32");
-    if (shift < 0 || shift > 62) return fail(MIND_B200_ERR_INVALID, "shift must be 0..62");
+    if (group <= 0 || group % 32 || group > MAX_DIM) return fail(MIND_B200_ERR_INVALID, "group must be a positive multiple of 32");
+    if (shift < 0 || shift > 28) return fail(MIND_B200_ERR_INVALID, "shift must be 0..28");
     if (!rows_of && x_rows != m) return fail(MIND_B200_ERR_INVALID, "without row indices x must have one row per output row");
     if (m == 0 || rows == 0 || experts == 0) return 0;
     const int es = kind == 0 ? 1 : (kind == 1 ? 2 : 4);

@@ -314,6 +314,15 @@ struct GroupedArgs {
     int shift, bt;
 };
 int64_t launch_gemm_grouped_i8(DeviceCtx* ctx, const GroupedArgs& g);
+// dst[i] = row idx[i] (idx null: i) of src, padded with zeros to `pitch` bytes (a multiple of 16); a row
+// outside [0, src_rows) is zeros.  A kernel launched behind it with programmatic serialization starts
+// when everything before the copy is complete, and must wait for the copy itself.
+int64_t launch_copy_rows(DeviceCtx* ctx, const int8_t* src, const int32_t* idx, int8_t* dst, int64_t rows, int64_t cols,
+                         int64_t pitch, int64_t src_rows);
+// Tensor map over `experts` row-major 8-bit matrices [rows][cols] of row pitch `pitch`, one behind the
+// other: boxes of 128 columns by box_rows rows in the 128-byte swizzle.  Cached per thread.
+int64_t make_tmap_stack(CUtensorMap* tm, const void* base, int64_t cols, int64_t rows, int64_t experts, int64_t pitch,
+                        int box_rows);
 int64_t launch_expert_plan(DeviceCtx* ctx, const int32_t* ids, int32_t* offsets, int32_t* rows, int32_t* place,
                            int64_t count, int64_t experts, int64_t per);
 int64_t launch_lcg_fill(DeviceCtx* ctx, void* dst, int64_t n, int kind, uint64_t seed,

@@ -130,6 +130,8 @@ copy_rows_kernel(const int8_t* __restrict__ src, const int32_t* __restrict__ idx
     }
 }
 
+}  // namespace
+
 int64_t launch_copy_rows(DeviceCtx* ctx, const int8_t* src, const int32_t* idx, int8_t* dst, int64_t rows, int64_t cols,
                          int64_t pitch, int64_t src_rows) {
     int64_t blocks = (rows + 7) / 8;
@@ -148,6 +150,7 @@ int64_t launch_copy_rows(DeviceCtx* ctx, const int8_t* src, const int32_t* idx, 
     return check_launch("copy_rows_kernel");
 }
 
+namespace {
 // ------------------------------------------------------------------ tensor cores
 constexpr int BLOCK_K = 128;  // bytes of K per stage
 constexpr int UMMA_K = 32;
@@ -501,6 +504,8 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
     }
 }
 
+}  // namespace
+
 // Map over a stack of `experts` row-major 8-bit matrices [rows][cols] of row pitch `pitch`: boxes of
 // 128 columns by box_rows rows in the 128-byte swizzle.  Reads past cols or rows return zeros.
 int64_t make_tmap_stack(CUtensorMap* tm, const void* base, int64_t cols, int64_t rows, int64_t experts, int64_t pitch,
@@ -544,6 +549,8 @@ int64_t make_tmap_stack(CUtensorMap* tm, const void* base, int64_t cols, int64_t
     if (cache.used < N) ++cache.used;
     return 0;
 }
+
+namespace {
 
 // a: pitch pa, b: pitch pb (both 16-byte multiples on 16-byte bases).
 template <int A_ROWS, int BLOCK_N, int PAIR, bool BMN>

@@ -3,12 +3,15 @@
 //   d[t,r,g] = sum_{k in group g} w[r,k] * x[t,k]            w in [-8, 7], x int8 / int16 / Q16.16
 //   y[t,r]   = (i32)( ( sum_g scale[r,g] * d[t,r,g] ) >> shift )
 //
-// The sum over groups is taken mod 2^64 and is exact for every operand a model holds
-// (|sum| < 2^49 * cols for Q16.16, 2^33 * cols for int16, 2^25 * cols for int8); it is shifted
+// The sum over groups is taken mod 2^64 (the low 60 bits decide the output; a model's sums are far smaller:
+// |sum| < 2^49 * cols for Q16.16, 2^33 * cols for int16, 2^25 * cols for int8); it is shifted
 // once and truncated once, so any order of accumulation gives the same bits.
 //
 // Weights: two a byte, the even column in the low half, rows of ceil(cols / 2) bytes.
-#include "common.h"
+//
+// gemv_w4.cuh holds the kernel that runs by default; here are the choice of its shape, the operands
+// it cannot address, and the cross-check kernel.
+#include "gemv_w4.cuh"
 
 namespace mb200 {
 namespace {
@@ -60,9 +63,65 @@ gemv_w4_warp_kernel(const W4Args a) {
     }
 }
 
-}  // namespace
+// How a call runs on the tensor-core kernel: blocks of at most tb tokens, clusters of cs blocks over the
+// columns, rt row tiles to a round.  Every choice gives the same bytes; the one with the least estimated
+// time is taken.  The estimate is in clocks of the busiest block: its share of the memory traffic, or its
+// instructions and the fixed cost of its rounds, whichever is more, and the activations' layout.
+bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int nt, w4::Plan* out) {
+    const int L = a.kind == 0 ? 1 : (a.kind == 1 ? 2 : 4);
+    const int ac = 8 * (nt ? nt : 1);
+    const int kb_total = (int)((a.cols + w4::KB - 1) / w4::KB);
+    const size_t table = align_up((size_t)(a.experts + 1) * 8, 128);
+    const double tiles = nt ? (double)L * ((tb + 7) / 8) : 2.0;  // MMAs per 32 columns
+    const double unit = 16.0 * (70.0 + 8.0 * (10.0 + 3.0 * tiles)) / 4.0;  // issue slots of 16 units on four schedulers
+    const int64_t blocks = a.offsets ? (a.m + tb - 1) / tb + (a.experts < a.m ? a.experts : a.m) / 2 : (a.m + tb - 1) / tb;
+    double best = 0;
+    for (int cs = 1; cs <= 8; cs *= 2) {
+        if (cs > kb_total) break;
+        const int fit = w4::cluster_fit(ctx, cs);
+        if (fit < 1) continue;
+        const int kb_slice = (kb_total + cs - 1) / cs;
+        const size_t x_bytes = (size_t)kb_slice * w4::KB * L * tb;
+        for (int rl = 0; rl <= 4; ++rl) {
+            const int rt = 1 << rl;
+            const size_t part = (size_t)w4::WARPS * 16 * ac * 8;
+            const size_t sums = cs > 1 ? align_up((size_t)2 * cs * ((16 * rt * tb + cs - 1) / cs) * 8, 128) : 0;
+            const size_t fixed = 1024 + w4::HEAD_BYTES + part + sums + x_bytes + table;
+            if (fixed + 2 * w4::RING_BYTES > (size_t)w4::SMEM_MAX) continue;
+            int slots = (int)((w4::SMEM_MAX - fixed) / w4::RING_BYTES);
+            if (slots > w4::MAX_SLOTS) slots = w4::MAX_SLOTS;
+            const int64_t row_rounds = (a.rows + 16 * rt - 1) / (16 * rt);
+            const int64_t rounds = blocks * row_rounds;
+            if (rounds > 0x3fffffff) continue;
+            const int64_t clusters = rounds < fit ? rounds : fit;
+            const int64_t most = (rounds + clusters - 1) / clusters;  // rounds of the busiest cluster
+            const int wpr = w4::WARPS / rt, steps = (kb_slice + wpr - 1) / wpr;
+            const double active = (double)clusters * cs;
+            const double mem = (double)most * rt * kb_slice * w4::SLOT_BYTES * active / 3400.0;
+            const double work = (double)most * (steps * unit + (cs > 1 ? 700.0 : 350.0));
+            const double cost = (mem > work ? mem : work) + 0.2 * (mem > work ? work : mem) + x_bytes / 24.0;
+            if (best == 0 || cost < best) {
+                best = cost;
+                w4::Params& p = out->p;
+                p.kb_total = kb_total;
+                p.cs = cs;
+                p.rt_log2 = rl;
+                p.tb = tb;
+                p.slots = slots;
+                p.row_rounds = (int)row_rounds;
+                p.off_part = (uint32_t)(w4::HEAD_BYTES + slots * w4::RING_BYTES);
+                p.off_sums = p.off_part + (uint32_t)part;
+                p.off_x = p.off_sums + (uint32_t)sums;
+                p.off_table = p.off_x + (uint32_t)x_bytes;
+                out->grid = (int)(clusters * cs);
+                out->smem = (int)(1024 + p.off_table + table);
+            }
+        }
+    }
+    return best != 0;
+}
 
-int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
+int64_t launch_warp_kernel(DeviceCtx* ctx, const W4Args& a) {
     int64_t blocks = (a.m * a.rows + 7) / 8;
     if (blocks > (int64_t)ctx->sm_count * 64) blocks = (int64_t)ctx->sm_count * 64;
     prof_begin(ctx);
@@ -75,6 +134,50 @@ int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
     prof_end(ctx);
     count_launch();
     return check_launch("gemv_w4_warp_kernel");
+}
+
+}  // namespace
+
+int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
+    if (tuning().gemm_path.load() == 1 || a.cols == 0 || a.x_rows == 0) return launch_warp_kernel(ctx, a);
+    const int L = a.kind == 0 ? 1 : (a.kind == 1 ? 2 : 4);
+    // Tokens per block: all of them up to 32, in blocks of equal size beyond.  Of grouped rows the kernel
+    // learns the groups' sizes itself; twice the average leaves few experts with a second block.
+    int64_t want = a.m;
+    if (a.offsets) {
+        const int64_t twice = 2 * ((a.m + a.experts - 1) / a.experts) + 2;
+        if (want > twice) want = twice;
+    }
+    int64_t passes = (want + 31) / 32;
+    w4::Plan plan;
+    int nt = 0;
+    for (;; ++passes) {  // more blocks where the activations of one would not fit
+        const int tb = (int)((want + passes - 1) / passes);
+        nt = L > 1 && tb <= 8 / L ? 0 : tb <= 8 ? 1 : tb <= 16 ? 2 : 4;
+        if (make_plan(ctx, a, tb, nt, &plan)) break;
+        if (tb == 1) return launch_warp_kernel(ctx, a);  // a row of activations too long for eight blocks
+    }
+    // TMA reads rows whose pitch and base are multiples of 16 bytes; others are copied to padded rows first
+    const int64_t bytes = (a.cols + 1) / 2, pitch = (int64_t)align_up((size_t)bytes, 16);
+    const int8_t* w = a.w;
+    if (pitch != bytes || reinterpret_cast<uintptr_t>(w) % 16 != 0) {
+        const size_t size = (size_t)(a.experts * a.rows) * pitch;
+        MB200_TRY(arena_reserve(ctx, ctx->scratch, size + 2048));
+        int8_t* to = static_cast<int8_t*>(arena_take(ctx->scratch, size));
+        MB200_TRY(launch_copy_rows(ctx, w, nullptr, to, a.experts * a.rows, bytes, pitch, a.experts * a.rows));
+        w = to;
+    }
+    CUtensorMap tm;
+    MB200_TRY(make_tmap_stack(&tm, w, bytes, a.rows, a.experts, pitch, 16));
+    w4::Params& p = plan.p;
+    p.a = a;
+    p.groups = (int)((a.cols + a.group - 1) / a.group);
+    p.group32 = (int)(a.group / 32 > 0x3fffffff ? 0x40000000 : a.group / 32);
+    p.x_vec = a.cols % 8 == 0 && reinterpret_cast<uintptr_t>(a.x) % (L == 1 ? 8 : 16) == 0 ? 1 : 0;
+    p.err = ctx->err_word;
+    if (a.kind == 0) return w4::launch_i8(ctx, tm, plan, nt);
+    if (a.kind == 1) return w4::launch_i16(ctx, tm, plan, nt);
+    return w4::launch_q16(ctx, tm, plan, nt);
 }
 
 }  // namespace mb200
