@@ -16,6 +16,11 @@ from . import check, last_error, lib, MindB200Error
 
 def addr(x) -> int:
     """Raw address of a numpy array, a torch tensor, or an int passed through."""
+    if type(x) is int:
+        return x
+    ptr = getattr(x, "data_ptr", None)  # tensors first: launch-bound callers pass several per call
+    if ptr is not None and x.is_contiguous():
+        return ptr()
     if isinstance(x, (int, np.integer)):
         return int(x)
     if isinstance(x, np.ndarray):

@@ -13,6 +13,7 @@
 // it cannot address, and the cross-check kernel.
 #include "gemv_w4.cuh"
 
+
 namespace mb200 {
 namespace {
 
@@ -65,15 +66,22 @@ gemv_w4_warp_kernel(const W4Args a) {
 
 // How a call runs on the tensor-core kernel: blocks of at most tb tokens, clusters of cs blocks over the
 // columns, rt row tiles to a round.  Every choice gives the same bytes; the one with the least estimated
-// time is taken.  The estimate is in clocks of the busiest block: its share of the memory traffic, or its
-// instructions and the fixed cost of its rounds, whichever is more, and the activations' layout.
-bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int nt, w4::Plan* out) {
+// time is taken.  The estimate is in clocks of the busiest block.
+bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
     const int L = a.kind == 0 ? 1 : (a.kind == 1 ? 2 : 4);
-    const int ac = 8 * (nt ? nt : 1);
+    const int ac = tc <= 8 ? 8 : tc, tok8 = (tb + 7) / 8;
+    const bool pack = L > 1 && L * tc <= 8;
     const int kb_total = (int)((a.cols + w4::KB - 1) / w4::KB);
+    const int g32 = (int)(a.group / 32 % 4), gb = g32 == 0 ? 4 : (g32 == 2 ? 2 : 1);
     const size_t table = align_up((size_t)(a.experts + 1) * 8, 128);
-    const double tiles = nt ? (double)L * ((tb + 7) / 8) : 2.0;  // MMAs per 32 columns
-    const double unit = 16.0 * (70.0 + 8.0 * (10.0 + 3.0 * tiles)) / 4.0;  // issue slots of 16 units on four schedulers
+    const size_t part = align_up((size_t)w4::WARPS * 16 * (ac + 1) * 8, 1024);
+    // Instructions of a warp per unit, and the clocks of a unit that nothing overlaps
+    const double mmas = pack ? 2.0 : (double)L * tok8;                                     // per 32 columns
+    const double per32 = 8.0 + mmas + (pack ? 1.0 : mmas) * (gb == 1 ? 1.0 : 0.5) + (pack ? 4.0 : 0.0);
+    const double scaling = 8.0 + 4.0 * (pack ? 2.0 : (L == 4 ? 6.0 : L == 2 ? 3.0 : 2.0) * tok8);
+    const double unit = 110.0 + 16.0 * per32 + 16.0 / gb * scaling;
+    const double fill = 30.0 + 30.0 * L;                                                  // per eight activations
+    const int64_t tiles = (a.rows + 15) / 16;
     const int64_t blocks = a.offsets ? (a.m + tb - 1) / tb + (a.experts < a.m ? a.experts : a.m) / 2 : (a.m + tb - 1) / tb;
     double best = 0;
     for (int cs = 1; cs <= 8; cs *= 2) {
@@ -81,37 +89,43 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int nt, w4::Plan* out) {
         const int fit = w4::cluster_fit(ctx, cs);
         if (fit < 1) continue;
         const int kb_slice = (kb_total + cs - 1) / cs;
-        const size_t x_bytes = (size_t)kb_slice * w4::KB * L * tb;
-        for (int rl = 0; rl <= 4; ++rl) {
-            const int rt = 1 << rl;
-            const size_t part = (size_t)w4::WARPS * 16 * ac * 8;
-            const size_t sums = cs > 1 ? align_up((size_t)2 * cs * ((16 * rt * tb + cs - 1) / cs) * 8, 128) : 0;
-            const size_t fixed = 1024 + w4::HEAD_BYTES + part + sums + x_bytes + table;
-            if (fixed + 2 * w4::RING_BYTES > (size_t)w4::SMEM_MAX) continue;
-            int slots = (int)((w4::SMEM_MAX - fixed) / w4::RING_BYTES);
-            if (slots > w4::MAX_SLOTS) slots = w4::MAX_SLOTS;
-            const int64_t row_rounds = (a.rows + 16 * rt - 1) / (16 * rt);
-            const int64_t rounds = blocks * row_rounds;
+        const size_t x_bytes = (size_t)kb_slice * w4::KB * L * tc;
+        for (int rt = 1; rt <= w4::WARPS; ++rt) {
+            const int wpr = w4::WARPS / rt, steps = (kb_slice + wpr - 1) / wpr;
+            const int64_t row_rounds = (tiles + rt - 1) / rt, rounds = blocks * row_rounds;
             if (rounds > 0x3fffffff) continue;
             const int64_t clusters = rounds < fit ? rounds : fit;
             const int64_t most = (rounds + clusters - 1) / clusters;  // rounds of the busiest cluster
-            const int wpr = w4::WARPS / rt, steps = (kb_slice + wpr - 1) / wpr;
+            const bool once = most == 1 && !a.offsets;
+            const size_t fixed = 1024 + w4::HEAD_BYTES + (once ? 0 : part) + x_bytes + table;
+            if (fixed + 2 * w4::RING_BYTES > (size_t)w4::SMEM_MAX) continue;
+            int slots = (int)((w4::SMEM_MAX - fixed) / w4::RING_BYTES);
+            if (slots > w4::MAX_SLOTS) slots = w4::MAX_SLOTS;
+            if (once && (size_t)slots * w4::RING_BYTES < part) continue;
             const double active = (double)clusters * cs;
-            const double mem = (double)most * rt * kb_slice * w4::SLOT_BYTES * active / 3400.0;
-            const double work = (double)most * (steps * unit + (cs > 1 ? 700.0 : 350.0));
-            const double cost = (mem > work ? mem : work) + 0.2 * (mem > work ? work : mem) + x_bytes / 24.0;
+            const int warps = rt * (wpr < kb_slice ? wpr : kb_slice);
+            const double issue = unit * ((warps + 3) / 4) / 0.7, alone = 500.0 + unit * 1.5;
+            const double step = issue > alone ? issue : alone;
+            // the memory's share: all blocks together at 3400 bytes a clock, one at 60 at most
+            const double bytes = (double)rt * kb_slice * 4096.0;
+            const double mem = bytes * (active / 3400.0 > 1.0 / 60.0 ? active / 3400.0 : 1.0 / 60.0);
+            const double work = steps * step;
+            const double round = (mem > work ? mem : work) + 0.15 * (mem > work ? work : mem) + (cs > 1 ? 2000.0 : 700.0);
+            const double cost = most * round + (double)kb_slice * w4::KB / 8 * tb / w4::THREADS * fill * 4 / 0.7;
             if (best == 0 || cost < best) {
                 best = cost;
                 w4::Params& p = out->p;
                 p.kb_total = kb_total;
                 p.cs = cs;
-                p.rt_log2 = rl;
+                p.cs_log2 = cs == 8 ? 3 : cs / 2;
+                p.rt = rt;
                 p.tb = tb;
                 p.slots = slots;
                 p.row_rounds = (int)row_rounds;
-                p.off_part = (uint32_t)(w4::HEAD_BYTES + slots * w4::RING_BYTES);
-                p.off_sums = p.off_part + (uint32_t)part;
-                p.off_x = p.off_sums + (uint32_t)sums;
+                p.once = once ? 1 : 0;
+                const uint32_t ring_end = (uint32_t)(w4::HEAD_BYTES + slots * w4::RING_BYTES);
+                p.off_part = once ? (uint32_t)w4::HEAD_BYTES : ring_end;
+                p.off_x = ring_end + (once ? 0 : (uint32_t)part);
                 p.off_table = p.off_x + (uint32_t)x_bytes;
                 out->grid = (int)(clusters * cs);
                 out->smem = (int)(1024 + p.off_table + table);
@@ -150,11 +164,11 @@ int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
     }
     int64_t passes = (want + 31) / 32;
     w4::Plan plan;
-    int nt = 0;
+    int tc = 1;
     for (;; ++passes) {  // more blocks where the activations of one would not fit
         const int tb = (int)((want + passes - 1) / passes);
-        nt = L > 1 && tb <= 8 / L ? 0 : tb <= 8 ? 1 : tb <= 16 ? 2 : 4;
-        if (make_plan(ctx, a, tb, nt, &plan)) break;
+        for (tc = 1; tc < tb;) tc *= 2;
+        if (make_plan(ctx, a, tb, tc, &plan)) break;
         if (tb == 1) return launch_warp_kernel(ctx, a);  // a row of activations too long for eight blocks
     }
     // TMA reads rows whose pitch and base are multiples of 16 bytes; others are copied to padded rows first
@@ -173,11 +187,16 @@ int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
     p.a = a;
     p.groups = (int)((a.cols + a.group - 1) / a.group);
     p.group32 = (int)(a.group / 32 > 0x3fffffff ? 0x40000000 : a.group / 32);
+    const int gb = p.group32 % 4 == 0 ? 4 : (p.group32 % 2 == 0 ? 2 : 1), ns = w4::KB / 128 / gb;
+    p.group_shift = -1;
+    for (int i = 0; i < 31; ++i)
+        if (p.group32 == 1 << i) p.group_shift = i;
+    p.scale_vec = p.group32 == gb && p.groups % ns == 0 && reinterpret_cast<uintptr_t>(a.scale) % (2 * ns) == 0 ? 1 : 0;
     p.x_vec = a.cols % 8 == 0 && reinterpret_cast<uintptr_t>(a.x) % (L == 1 ? 8 : 16) == 0 ? 1 : 0;
     p.err = ctx->err_word;
-    if (a.kind == 0) return w4::launch_i8(ctx, tm, plan, nt);
-    if (a.kind == 1) return w4::launch_i16(ctx, tm, plan, nt);
-    return w4::launch_q16(ctx, tm, plan, nt);
+    if (a.kind == 0) return w4::launch_i8(ctx, tm, plan, tc);
+    if (a.kind == 1) return w4::launch_i16(ctx, tm, plan, tc);
+    return w4::launch_q16(ctx, tm, plan, tc);
 }
 
 }  // namespace mb200

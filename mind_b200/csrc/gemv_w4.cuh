@@ -9,17 +9,20 @@
 // * Activations become columns of bytes: x = sum_i limb_i * 256^i, all but the top limb unsigned.  With
 //   few tokens one set of accumulators holds all limbs as columns (PACK: two MMAs, unsigned and signed
 //   columns, the other ones zero); with more, eight tokens and one limb make an MMA.
-// * Weights arrive as they lie, 16 rows x 256 columns at a time, by TMA into a ring of 2 KiB slots that
+// * Weights arrive as they lie, in boxes of 16 rows x 256 columns, by TMA into a ring of 2 KiB slots that
 //   each warp keeps for itself: no barrier between warps in the main loop.  A word of eight weights
 //   becomes two registers of four by masking, as 16 times the weight: the factor leaves with the final
-//   shift.  The columns 32 j + 8 t + {0,2,4,6} / {1,3,5,7} go where the MMA has k = 4 t + {0..3} /
-//   16 + 4 t + {0..3}; the activations are laid out in shared memory in that order once per block.
-// * After GB x 32 columns (a divisor of the group, at most 128 columns) the int32 sums are multiplied by
-//   the group's scale and added up in 64 bits, in registers.
-// * 16 warps share `rt` row tiles, 16 / rt warps to a tile, which take its 256-column blocks in turn; a
+//   shift.
+// * After GB x 32 columns (GB = 4, 2 or 1: a divisor of the group) the int32 sums are multiplied by the
+//   group's scale and added up in 64 bits, in registers.  Lane t of a row's four takes GB consecutive
+//   words of those columns with one load, and the MMAs take the words in turn: MMA i has the columns
+//   8 GB t + 8 i + {0,2,4,6} / {1,3,5,7} at its k = 4 t + {0..3} / 16 + 4 t + {0..3}.  The activations
+//   are laid out in shared memory in that order, once per block of tokens.
+// * 16 warps share `rt` row tiles, 16 / rt warps to a tile, which take its units of 512 columns in turn; a
 //   cluster of up to eight blocks shares the columns where a block's activations would not fit beside
-//   the ring.  Partial sums meet in shared memory (across the cluster, too): integer sums, so no order
-//   of arrival changes a bit, and nothing is kept in global memory.
+//   the ring, or where there are fewer row tiles than warps.  The partial sums meet in shared memory,
+//   across the cluster by remote reads: integer sums, so no order changes a bit, and nothing is kept in
+//   global memory.
 #pragma once
 #include "common.h"
 #include "ptx.cuh"
@@ -29,108 +32,142 @@ namespace w4 {
 using namespace ptx;
 
 constexpr int WARPS = 16, THREADS = 32 * WARPS;
-constexpr int SLOT_BYTES = 2048;                    // 16 rows x 128 bytes
-constexpr int RING_BYTES = WARPS * SLOT_BYTES;      // one slot of every warp
-constexpr int KB = 256;                             // columns of a slot
+constexpr int BOX_BYTES = 2048;                     // 16 rows x 128 bytes: one TMA box
+constexpr int RING_BYTES = WARPS * BOX_BYTES;       // one slot of every warp
+constexpr int KB = 512;                             // columns of a unit: two boxes
 constexpr int SMEM_MAX = 232448;
 constexpr int MAX_SLOTS = 8;
 constexpr int HEAD_BYTES = 2048;                    // barriers and scan scratch
 
 struct Params {
     W4Args a;
-    int kb_total;         // 256-column blocks
-    int cs, rt_log2;      // cluster size; row tiles per round
+    int kb_total;         // units of 512 columns
+    int cs, cs_log2, rt;  // cluster size; row tiles per round
     int tb;               // tokens per block, at most
-    int slots;            // ring depth
+    int slots;            // ring depth, in boxes
     int row_rounds;       // rounds of 16 * rt rows per matrix
+    int once;             // no cluster has more than one round: the partial sums take the ring's place
     int groups, group32;  // groups per row; 32-column blocks per group
+    int group_shift;      // log2 of group32, or -1
     int x_vec;            // x may be read eight elements at a time
-    uint32_t off_part, off_sums, off_x, off_table;  // shared-memory layout, from the aligned base
+    int scale_vec;        // a group is one scaling, and a lane's scales of a unit are one aligned load
+    uint32_t off_part, off_x, off_table;  // shared-memory layout, from the aligned base
     int* err;
 };
 
-struct Cursor {  // one unit of a warp: row tile and 256-column block
-    int u, kb, e, row0;
+// D (+)= A . B, 16 x 32 weights (s8) by 32 x 8 activation bytes.  FIRST: D = A . B.  KEEP: stays before
+// every later volatile statement (the refill of the slot that its operands came from).
+template <bool SIGNED, bool FIRST, bool KEEP>
+__device__ __forceinline__ void mma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+#define MB200_W4_MMA(V, T, C, ...)                                                                                          \
+    asm V("mma.sync.aligned.m16n8k32.row.col.s32.s8." T ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " C ";" __VA_ARGS__)
+#define MB200_W4_IN "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1)
+#define MB200_W4_NEW : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : MB200_W4_IN, "r"(0)
+#define MB200_W4_ADD : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : MB200_W4_IN
+    if constexpr (SIGNED && FIRST && KEEP) MB200_W4_MMA(volatile, "s8", "{%10,%10,%10,%10}", MB200_W4_NEW);
+    else if constexpr (SIGNED && FIRST) MB200_W4_MMA(, "s8", "{%10,%10,%10,%10}", MB200_W4_NEW);
+    else if constexpr (SIGNED && KEEP) MB200_W4_MMA(volatile, "s8", "{%0,%1,%2,%3}", MB200_W4_ADD);
+    else if constexpr (SIGNED) MB200_W4_MMA(, "s8", "{%0,%1,%2,%3}", MB200_W4_ADD);
+    else if constexpr (FIRST && KEEP) MB200_W4_MMA(volatile, "u8", "{%10,%10,%10,%10}", MB200_W4_NEW);
+    else if constexpr (FIRST) MB200_W4_MMA(, "u8", "{%10,%10,%10,%10}", MB200_W4_NEW);
+    else if constexpr (KEEP) MB200_W4_MMA(volatile, "u8", "{%0,%1,%2,%3}", MB200_W4_ADD);
+    else MB200_W4_MMA(, "u8", "{%0,%1,%2,%3}", MB200_W4_ADD);
+#undef MB200_W4_MMA
+#undef MB200_W4_IN
+#undef MB200_W4_NEW
+#undef MB200_W4_ADD
+}
+template <bool SIGNED>
+__device__ __forceinline__ void mma_step(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first, bool keep) {
+    if (first && keep) mma<SIGNED, true, true>(d, a, b0, b1);
+    else if (first) mma<SIGNED, true, false>(d, a, b0, b1);
+    else if (keep) mma<SIGNED, false, true>(d, a, b0, b1);
+    else mma<SIGNED, false, false>(d, a, b0, b1);
+}
+// 4 * N bytes of shared memory.
+template <int N>
+__device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t addr) {
+    if constexpr (N == 4)
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+    else if constexpr (N == 2)
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr) : "memory");
+    else
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[0]) : "r"(addr) : "memory");
+}
+// Bytes of activations of one column that lane t holds for GB MMAs: in pieces of at most 16, so that
+// the lanes of a load lie side by side.
+template <int GB>
+struct XPiece {
+    static constexpr int BYTES = GB == 1 ? 8 : 16, PIECES = 8 * GB / BYTES, MMAS = BYTES / 8;
 };
 
-__device__ __forceinline__ void mma_s8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool zero) {
-    if (zero)
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
-    else
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma_s8u8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool zero) {
-    if (zero)
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
-                     : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
-    else
-        asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                     : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
-                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-    return v;
-}
-
-// Eight activations k .. k + 7 of row xr as int32 (zeros past the end).
+// Eight activations k .. k + 7 of row xr as they lie in memory, 2 * L words (zeros past the end).
 template <int L>
-__device__ __forceinline__ void load8(const Params& p, int64_t xr, int64_t k, int32_t (&v)[8]) {
-    const int64_t at = xr * p.a.cols + k;
+__device__ __forceinline__ void load8(const Params& p, int64_t xr, int64_t k, uint32_t (&v)[2 * L]) {
+    const char* const at = static_cast<const char*>(p.a.x) + (xr * p.a.cols + k) * L;
     if (p.x_vec && k + 8 <= p.a.cols) {
-        if (L == 1) {
-            const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const int8_t*>(p.a.x) + at);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[i] = (int32_t)(w.x << (24 - 8 * i)) >> 24;
-                v[i + 4] = (int32_t)(w.y << (24 - 8 * i)) >> 24;
-            }
-        } else if (L == 2) {
-            const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const int16_t*>(p.a.x) + at);
-            const uint32_t s[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = (int32_t)(s[i] << 16) >> 16;
-                v[2 * i + 1] = (int32_t)s[i] >> 16;
-            }
+        if constexpr (L == 1) {
+            const uint2 w = *reinterpret_cast<const uint2*>(at);
+            v[0] = w.x;
+            v[1] = w.y;
         } else {
-            const int4 lo = *reinterpret_cast<const int4*>(static_cast<const int32_t*>(p.a.x) + at);
-            const int4 hi = *reinterpret_cast<const int4*>(static_cast<const int32_t*>(p.a.x) + at + 4);
-            v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
-            v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
+#pragma unroll
+            for (int i = 0; i < L / 2; ++i) {
+                const uint4 w = *reinterpret_cast<const uint4*>(at + 16 * i);
+                v[4 * i] = w.x;
+                v[4 * i + 1] = w.y;
+                v[4 * i + 2] = w.z;
+                v[4 * i + 3] = w.w;
+            }
         }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = 0;
-        if (k + i < p.a.cols)
-            v[i] = L == 1 ? static_cast<const int8_t*>(p.a.x)[at + i]
-                          : L == 2 ? static_cast<const int16_t*>(p.a.x)[at + i] : static_cast<const int32_t*>(p.a.x)[at + i];
+    for (int i = 0; i < 2 * L; ++i) v[i] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (k + i < p.a.cols) {
+            if constexpr (L == 1) v[i / 4] |= (uint32_t)*reinterpret_cast<const uint8_t*>(at + i) << (8 * (i % 4));
+            else if constexpr (L == 2) v[i / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(at + 2 * i) << (16 * (i % 2));
+            else v[i] = *reinterpret_cast<const uint32_t*>(at + 4 * i);
+        }
+}
+// Limb l of the activations 0, 2, 4, 6 (odd = 0) or 1, 3, 5, 7 (odd = 1) of such words.
+template <int L>
+__device__ __forceinline__ uint32_t limb4(const uint32_t (&v)[2 * L], int l, int odd) {
+    if constexpr (L == 1) return __byte_perm(v[0], v[1], odd ? 0x7531 : 0x6420);
+    if constexpr (L == 2) {
+        const uint32_t sel = (l + 2 * odd) | ((l + 2 * odd + 4) << 4);
+        return __byte_perm(__byte_perm(v[0], v[1], sel), __byte_perm(v[2], v[3], sel), 0x5410);
+    } else if constexpr (L == 4) {
+        const uint32_t sel = l | ((l + 4) << 4);
+        return __byte_perm(__byte_perm(v[odd], v[2 + odd], sel), __byte_perm(v[4 + odd], v[6 + odd], sel), 0x5410);
     }
+    return 0;
+}
+// The rest of a wait that did not end at once.
+static __device__ __noinline__ bool wait_on(uint32_t bar, uint32_t parity, volatile int* abort_s, int* err) {
+    return wait_bounded(bar, parity, abort_s, err, 5);
 }
 
-// L: limbs of an activation (1 = int8, 2 = int16, 4 = Q16.16).  NT: blocks of eight tokens.  PACK: all
-// limbs of 8 / L tokens in one set of accumulators.  GB: 32-column blocks between two scalings.
-template <int L, int NT, bool PACK, int GB>
-__global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ CUtensorMap tm_w, const Params p) {
-    static_assert(!PACK || (NT == 1 && L > 1), "packing is for few tokens of several limbs");
+// L: limbs of an activation (1 = int8, 2 = int16, 4 = Q16.16).  TC: tokens that a block has room for (the
+// layout of the activations, and with it every address of the main loop, is fixed by it).  GB: 32-column
+// blocks between two scalings.
+template <int L, int TC, int GB>
+__global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_constant__ CUtensorMap tm_w, const Params p) {
+    constexpr bool PACK = L > 1 && L * TC <= 8;  // all limbs of the tokens in one set of accumulators
+    constexpr int NT = (TC + 7) / 8;      // blocks of eight tokens
     constexpr int LT = PACK ? 1 : L;      // accumulator sets between scalings
     constexpr int AC = 8 * NT;            // accumulator columns of a warp
+    constexpr int PS = AC + 1;            // stride of a row of partial sums: rows side by side hit different banks
     constexpr int TP = PACK ? 8 / L : 1;  // tokens per limb in a packed set
-    constexpr int NF = 8 / GB;            // scalings per slot
-    constexpr int NS = (NF + 3) / 4;      // scale registers per lane and row
+    constexpr int NF = KB / 32 / GB;      // scalings per unit
+    constexpr int FB = NF / 2;            // per box
+    constexpr int NS = NF / 4;            // of which every lane of four holds NS consecutive ones
+    using XP = XPiece<GB>;
+    constexpr int XCOLS = L * TC;              // columns of activation bytes
+    constexpr int CSTRIDE = XCOLS * 32 * GB;   // bytes of the activations between two scalings
+    constexpr int LIMB_STRIDE = TC * 4 * XP::BYTES, PIECE_STRIDE = XCOLS * 4 * XP::BYTES;
 
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -138,17 +175,20 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ CUt
     const uint32_t ring0 = base + HEAD_BYTES;
     int* const misc = reinterpret_cast<int*>(gbase + WARPS * MAX_SLOTS * 8);
     volatile int* const abort_s = misc;
-    uint64_t* const part = reinterpret_cast<uint64_t*>(gbase + p.off_part);  // [warp][16][AC]
-    uint64_t* const sums = reinterpret_cast<uint64_t*>(gbase + p.off_sums);  // [2][cs][outputs / cs]
+    uint64_t* const part = reinterpret_cast<uint64_t*>(gbase + p.off_part);  // [warp][16][PS]
     const uint32_t xs = base + p.off_x;
     int* const bound = reinterpret_cast<int*>(gbase + p.off_table);  // [experts + 1] first row of each
     int* const cumb = bound + p.a.experts + 1;                       // [experts + 1] token blocks before each
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rt = 1 << p.rt_log2, wpr = WARPS >> p.rt_log2;
+    // The row of the tile that MMA row g stands for: with its bits reversed the lanes of one phase of a
+    // load fall on different 16-byte columns of the swizzled box, whatever GB.
+    const int row = ((g & 1) << 2) | (g & 2) | (g >> 2);
+    const int rt = p.rt, wpr = WARPS / rt;       // warps beyond rt * wpr only help with the activations
+    const int my_tile = warp % rt, my_part = warp / rt;
     const uint32_t rank = p.cs > 1 ? cluster_ctarank() : 0u;
     const int clusters = gridDim.x / p.cs, cluster = blockIdx.x / p.cs;
-    const uint32_t bars = base + warp * MAX_SLOTS * 8, slots0 = ring0 + warp * SLOT_BYTES;
+    const uint32_t bars = base + warp * MAX_SLOTS * 8, slots0 = ring0 + warp * BOX_BYTES;
 
     griddep_launch_dependents();
     if (lane == 0)
@@ -158,13 +198,21 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ CUt
         prefetch_tensormap(&tm_w);
     }
     if (lane == 0) fence_mbar_init();
-    griddep_wait();  // from here on global memory is read
+    // Before the wait for the kernel in front nothing may be read that it could have written: grouped rows
+    // wait here, for their offsets; one matrix waits behind the set-up.
+    if (p.a.offsets) griddep_wait();
 
     // ---- token blocks: bound = running maximum of the offsets within [0, m], cumb = running sum of
     // the blocks of at most tb rows
-    {
+    if (!p.a.offsets) {
+        if (threadIdx.x == 0) {
+            bound[0] = cumb[0] = 0;
+            bound[1] = (int)p.a.m;
+            cumb[1] = ((int)p.a.m + p.tb - 1) / p.tb;
+        }
+    } else {
         const int experts = (int)p.a.experts, m = (int)p.a.m;
-        auto offset = [&](int e) { return p.a.offsets ? min(max(p.a.offsets[e], 0), m) : (e ? m : 0); };
+        auto offset = [&](int e) { return min(max(p.a.offsets[e], 0), m); };
         const int per = (experts + THREADS - 1) / THREADS;
         const int e0 = min((int)threadIdx.x * per, experts), e1 = min(e0 + per, experts);
         const int first = offset(0);
@@ -207,110 +255,161 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ CUt
             bound[0] = first;
             cumb[0] = 0;
         }
-        __syncthreads();
-        if (p.cs > 1) {  // every block of the cluster is running before any writes into another
-            cluster_arrive();
-            cluster_wait();
-        }
+    }
+    __syncthreads();
+    if (p.cs > 1) {  // every block of the cluster is running before any writes into another
+        cluster_arrive();
+        cluster_wait();
     }
     // Rounds (token block, 16 * rt rows) are handed out in equal runs, one run to a cluster.
-    const int64_t rounds = (int64_t)cumb[p.a.experts] * p.row_rounds;
-    const int u0 = (int)(rounds * cluster / clusters), u1 = (int)(rounds * (cluster + 1) / clusters);
-    const int kb_lo = (int)((int64_t)p.kb_total * rank / p.cs), kb_hi = (int)((int64_t)p.kb_total * (rank + 1) / p.cs);
-    const int kb_first = kb_lo + (warp >> p.rt_log2);
+    const unsigned rounds = (unsigned)cumb[p.a.experts] * (unsigned)p.row_rounds;
+    const unsigned run = rounds / (unsigned)clusters, more = rounds - run * (unsigned)clusters;
+    const int u0 = (int)(run * cluster + min((unsigned)cluster, more)), u1 = u0 + (int)run + ((unsigned)cluster < more ? 1 : 0);
+    const int kb_lo = (int)((unsigned)p.kb_total * rank >> p.cs_log2), kb_hi = (int)((unsigned)p.kb_total * (rank + 1) >> p.cs_log2);
+    const int kb_first = my_part < wpr ? kb_lo + my_part : kb_hi;
     const uint64_t policy = l2_policy(0);
 
-    auto place = [&](Cursor& c) {  // expert and row tile of round c.u
-        const int q = c.u / p.row_rounds;
-        while (q >= cumb[c.e + 1]) ++c.e;
-        c.row0 = (((c.u - q * p.row_rounds) << p.rt_log2) + (warp & (rt - 1))) * 16;
+    // This warp's units of a round: columns kb_first, kb_first + wpr, ...  Its boxes, in order: two a unit, but
+    // for a last unit that ends in its first.
+    const int steps = kb_first < kb_hi ? (kb_hi - kb_first + wpr - 1) / wpr : 0;
+    const int boxes = 2 * steps - (steps && (int64_t)(kb_first + (steps - 1) * wpr) * KB + KB / 2 >= p.a.cols ? 1 : 0);
+    auto group_of = [&](int blk) { return p.group_shift >= 0 ? blk >> p.group_shift : blk / p.group32; };
+    // the scales of row r of expert e (rows past the end meet zero weights: any scale will do)
+    auto scale_row = [&](int e, int r) {
+        return p.a.scale + ((int64_t)e * p.a.rows + min((int64_t)r, p.a.rows - 1)) * p.groups;
     };
-    auto advance = [&](Cursor& c) {
-        c.kb += wpr;
-        if (c.kb >= kb_hi) {
-            c.kb = kb_first;
-            if (++c.u < u1) place(c);
-        }
+    bool lead = lane == 0;  // asks for the boxes; nobody does any more once a wait has run out
+
+    int is_u = boxes ? u0 : u1, is_e = 0, is_row0 = 0, is_box = 0, is_x = kb_first * (KB / 2), fill = 0;  // next load
+    auto place = [&]() {
+        const int q = (int)((unsigned)is_u / (unsigned)p.row_rounds);
+        while (q >= cumb[is_e + 1]) ++is_e;
+        is_row0 = ((is_u - q * p.row_rounds) * rt + my_tile) * 16;
     };
-    Cursor is = {kb_first < kb_hi ? u0 : u1, kb_first, 0, 0}, nx = is;
-    if (is.u < u1) place(is);
-    nx = is;
-    int fill = 0;  // slot of the next load
     auto issue = [&]() {
-        if (is.u >= u1) return;
-        if (lane == 0 && !*abort_s) {
-            mbar_arrive_expect_tx(bars + 8 * fill, SLOT_BYTES);
-            tma_load_3d(slots0 + fill * RING_BYTES, &tm_w, bars + 8 * fill, is.kb * (KB / 2), is.row0, is.e, policy);
+        if (is_u >= u1) return;
+        if (lead) {
+            mbar_arrive_expect_tx(bars + 8 * fill, BOX_BYTES);
+            tma_load_3d(slots0 + fill * RING_BYTES, &tm_w, bars + 8 * fill, is_x, is_row0, is_e, policy);
         }
-        if (++fill == p.slots) fill = 0;
-        advance(is);
+        fill = fill + 1 == p.slots ? 0 : fill + 1;
+        if (++is_box == boxes) {
+            is_box = 0;
+            is_x = kb_first * (KB / 2);
+            if (++is_u < u1) place();
+        } else {
+            is_x += (is_box & 1) ? 128 : wpr * (KB / 2) - 128;
+        }
     };
-    for (int s = 0; s < p.slots; ++s) issue();
+    if (is_u < u1) place();
+    // A round's scales, towards L2: the warps of a row tile share the sectors of its rows.
+    auto prefetch_scales = [&](int u, int e) {
+        const int q = (int)((unsigned)u / (unsigned)p.row_rounds);
+        while (q >= cumb[e + 1]) ++e;
+        const int r = ((u - q * p.row_rounds) * rt + my_tile) * 16 + row;
+        const int g0 = group_of(kb_lo * (KB / 32)), g1 = min(group_of(kb_hi * (KB / 32) - 1), p.groups - 1);
+        const int16_t* const a0 = scale_row(e, r);
+        const int16_t* const a8 = scale_row(e, r + 8);
+        for (int gi = g0 + (my_part * 4 + t) * 16; gi <= g1 + 15 && my_part < wpr; gi += wpr * 64) {
+            const int at = min(gi, g1);
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(a0 + at));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(a8 + at));
+        }
+    };
 
-    // scales of a unit: lane t holds those of scalings t and t + 4, for rows g and g + 8
+    // Scales of a unit: lane t holds those of scalings t * NS .. t * NS + NS - 1, of two rows.  (Past the last
+    // group the weights are zeros, and the last scales are as good as any.)
     int sc0[NS], sc1[NS];
-    auto load_scales = [&](const Cursor& c) {
+    auto load_scales = [&](const int16_t* s, const int16_t* s8, int kb) {
+        if (p.scale_vec) {  // a group is one scaling, and a lane's are one aligned load
+            const int gi = min(kb * NF + t * NS, p.groups - NS);
+            auto fetch = [&](const int16_t* q, int (&sc)[NS]) {
+                if constexpr (NS == 1) {
+                    sc[0] = __ldg(q);
+                } else if constexpr (NS == 2) {
+                    const int v = __ldg(reinterpret_cast<const int*>(q));
+                    sc[0] = (int)(int16_t)v;
+                    sc[1] = v >> 16;
+                } else {
+                    const int2 v = __ldg(reinterpret_cast<const int2*>(q));
+                    sc[0] = (int)(int16_t)v.x;
+                    sc[1] = v.x >> 16;
+                    sc[2] = (int)(int16_t)v.y;
+                    sc[3] = v.y >> 16;
+                }
+            };
+            fetch(s + gi, sc0);
+            fetch(s8 + gi, sc1);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const int f = t + 4 * i, gi = (c.kb * 8 + f * GB) / p.group32, r = c.row0 + g;
-            const bool ok = f < NF && gi < p.groups && c.u < u1;
-            const int16_t* const s = p.a.scale + ((int64_t)c.e * p.a.rows + r) * p.groups + gi;
-            sc0[i] = ok && r < p.a.rows ? __ldg(s) : 0;
-            sc1[i] = ok && r + 8 < p.a.rows ? __ldg(s + 8 * (int64_t)p.groups) : 0;
+            for (int i = 0; i < NS; ++i) {
+                const int gi = min(group_of(kb * (KB / 32) + (t * NS + i) * GB), p.groups - 1);
+                sc0[i] = __ldg(s + gi);
+                sc1[i] = __ldg(s8 + gi);
+            }
         }
     };
-    load_scales(nx);
 
-    const int cstride = L * p.tb * 32;  // bytes of one 32-column block of activations
-    const uint32_t g7 = (uint32_t)(g & 7);
     int take = 0;
     uint32_t phase = 0;
     int block = -1, ntok = 0, p0 = 0, e_now = 0;
-    bool pending = false;       // a round's sums are on their way through the cluster
-    int pend_row0 = 0, pend_ntok = 0, pend_p0 = 0;
-    uint32_t pend_buf = 0, buf = 0;
     const int rows_round = 16 * rt;
 
-    auto finish_pending = [&]() {  // this block's share of the last round's outputs: add up the cluster's sums
-        cluster_wait();
-        const int outs = rows_round * pend_ntok;
-        const int per_rank = (rows_round * p.tb + p.cs - 1) / p.cs;
-        for (int i = threadIdx.x; i * p.cs + (int)rank < outs; i += THREADS) {
-            const int o = i * p.cs + (int)rank, r = pend_row0 + o % rows_round, tok = o / rows_round;
-            uint64_t s = 0;
-            for (int c = 0; c < p.cs; ++c) s += sums[(pend_buf * p.cs + c) * per_rank + i];
-            if (r < p.a.rows) p.a.y[(int64_t)(pend_p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)s >> (p.a.shift + 4));
-        }
-        pending = false;
-    };
-
+    if (!p.a.offsets) griddep_wait();
+    bool asked = false;  // the ring's first loads go out behind the first loads of activations
     for (int u = u0; u < u1; ++u) {
-        const int q = u / p.row_rounds;
+        const int q = (int)((unsigned)u / (unsigned)p.row_rounds);
         if (q != block) {
             // ---- a new block of tokens: its activations, as bytes in the order the MMAs take them
             block = q;
             while (q >= cumb[e_now + 1]) ++e_now;
-            const int nb = cumb[e_now + 1] - cumb[e_now], i = q - cumb[e_now];
-            const int64_t rows_e = bound[e_now + 1] - bound[e_now];
-            p0 = bound[e_now] + (int)(rows_e * i / nb);
-            ntok = bound[e_now] + (int)(rows_e * (i + 1) / nb) - p0;
+            const unsigned nb = cumb[e_now + 1] - cumb[e_now], i = q - cumb[e_now];
+            const unsigned rows_e = bound[e_now + 1] - bound[e_now], per = rows_e / nb, extra = rows_e - per * nb;
+            p0 = bound[e_now] + (int)(i * per + min(i, extra));
+            ntok = (int)per + (i < extra ? 1 : 0);
+            // A thread owns groups of eight columns and takes them token by token (several tokens at once where
+            // the columns are few), a batch of loads before the first store.
             const int octs = (kb_hi - kb_lo) * (KB / 8);
-            for (int tok = 0; tok < ntok; ++tok) {
-                const int64_t xr = p.a.rows_of ? p.a.rows_of[p0 + tok] : p0 + tok;
-                const bool inside = xr >= 0 && xr < p.a.x_rows;
-                for (int o = threadIdx.x; o < octs; o += THREADS) {
-                    int32_t v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-                    if (inside) load8<L>(p, xr, (int64_t)kb_lo * KB + 8 * o, v);
-                    const uint32_t at = xs + (o >> 2) * cstride + tok * 32 + (o & 3) * 8;
+            const int width = octs < THREADS ? octs : THREADS, tstep = THREADS / width;
+            const int tok0 = (int)threadIdx.x / width;
+            constexpr int BATCH = L == 4 ? 4 : 8;
+            for (int o = (int)threadIdx.x - tok0 * width; o < octs && tok0 < tstep; o += width) {
+                const int m = o % GB;  // MMA that takes these eight columns
+                const uint32_t at = xs + o / (4 * GB) * CSTRIDE + (m / XP::MMAS) * PIECE_STRIDE +
+                                    (o / GB & 3) * XP::BYTES + (m % XP::MMAS) * 8;
+                const int64_t k = (int64_t)kb_lo * KB + 8 * o;
+                for (int tk = tok0; tk < ntok; tk += BATCH * tstep) {
+                    uint32_t v[BATCH][2 * L];
 #pragma unroll
-                    for (int l = 0; l < L; ++l) {
-                        const uint32_t sel = l | ((l + 4) << 4);
-                        const uint32_t b0 = __byte_perm(__byte_perm(v[0], v[2], sel), __byte_perm(v[4], v[6], sel), 0x5410);
-                        const uint32_t b1 = __byte_perm(__byte_perm(v[1], v[3], sel), __byte_perm(v[5], v[7], sel), 0x5410);
-                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + l * p.tb * 32), "r"(b0), "r"(b1) : "memory");
+                    for (int b = 0; b < BATCH; ++b) {
+                        const int tok = tk + b * tstep;
+#pragma unroll
+                        for (int j = 0; j < 2 * L; ++j) v[b][j] = 0;
+                        if (tok >= ntok) break;
+                        const int64_t xr = p.a.rows_of ? p.a.rows_of[p0 + tok] : p0 + tok;
+                        if (xr >= 0 && xr < p.a.x_rows) load8<L>(p, xr, k, v[b]);
+                    }
+                    if (!asked) {
+                        asked = true;
+                        for (int s = 0; s < p.slots; ++s) issue();
+                    }
+#pragma unroll
+                    for (int b = 0; b < BATCH; ++b) {
+                        const int tok = tk + b * tstep;
+                        if (tok >= ntok) break;
+#pragma unroll
+                        for (int l = 0; l < L; ++l)
+                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + l * LIMB_STRIDE + tok * 4 * XP::BYTES),
+                                         "r"(limb4<L>(v[b], l, 0)), "r"(limb4<L>(v[b], l, 1))
+                                         : "memory");
                     }
                 }
             }
+            if (!asked) {
+                asked = true;
+                for (int s = 0; s < p.slots; ++s) issue();
+            }
+            if (u == u0) prefetch_scales(u0, e_now);
             __syncthreads();
         }
         // ---- this warp's units of the round
@@ -319,56 +418,73 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ CUt
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc64[n][i] = 0;
-        // packed: column g is limb g / TP of token g % TP
-        const bool col_ok = PACK ? g % TP < ntok : true;
+        // Packed: column g is limb g / TP of token g % TP.  A column without a token takes another's bytes
+        // (its sums are never looked at), so that no load is conditional.
         const bool col_top = PACK && g / TP == L - 1;
-        const uint32_t xcol = xs + (PACK ? ((g / TP) * p.tb + g % TP) * 32 : g * 32) + t * 8;
-        for (int kb = kb_first; kb < kb_hi; kb += wpr) {
-            int s0[NS], s1[NS];
+        int xtok[NT];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) xtok[n] = (PACK ? (g % TP < ntok ? g % TP : 0) : (n * 8 + g < ntok ? n * 8 + g : 0)) * 4 * XP::BYTES;
+        const uint32_t xcol = xs + (PACK ? g / TP : 0) * LIMB_STRIDE + t * XP::BYTES;
+        const int tile_row0 = ((u - q * p.row_rounds) * rt + my_tile) * 16;
+        const int16_t* const srow = scale_row(e_now, tile_row0 + row);
+        const int16_t* const srow8 = scale_row(e_now, tile_row0 + row + 8);
+        load_scales(srow, srow8, kb_first);
+        if (u + 1 < u1) prefetch_scales(u + 1, e_now);
+        uint32_t xnext = xcol + (kb_first - kb_lo) * NF * CSTRIDE;  // activations of the next scaling
+        for (int j = 0, kb = kb_first; j < steps; ++j, kb += wpr) {
+            int sc[2][NS];
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                s0[i] = sc0[i];
-                s1[i] = sc1[i];
+                sc[0][i] = sc0[i];
+                sc[1][i] = sc1[i];
             }
-            advance(nx);
-            load_scales(nx);
-            if (!*abort_s) wait_bounded(bars + 8 * take, phase, abort_s, p.err, 5);
-            __syncwarp();
-            const uint32_t wrow = slots0 + take * RING_BYTES + g * 128 + t * 4;
-            const uint32_t xblk = xcol + (kb - kb_lo) * 8 * cstride;
+            load_scales(srow, srow8, kb + wpr);
+            uint32_t xat = xnext;
+            xnext += wpr * NF * CSTRIDE;
 #pragma unroll
-            for (int f = 0; f < NF; ++f) {
-                const int m0 = __shfl_sync(0xffffffffu, s0[f >> 2], (lane & 28) | (f & 3));
-                const int m1 = __shfl_sync(0xffffffffu, s1[f >> 2], (lane & 28) | (f & 3));
-                uint32_t a[GB][4];
+            for (int h = 0; h < 2; ++h) {
+            if (h == 1 && 2 * j + 1 == boxes) break;
+            if (!mbar_try_wait(bars + 8 * take, phase)) lead = wait_on(bars + 8 * take, phase, abort_s, p.err) && lead;
+            // this lane's words of scaling f of the box lie at wbase ^ (f * 16 GB), the box's swizzle included
+            const uint32_t wbase = slots0 + take * RING_BYTES + row * 128 +
+                                   (((t * GB / 4) ^ row) << 4) + (t * GB % 4) * 4;
+#pragma unroll
+            for (int f = 0; f < FB; ++f) {
+                const int m0 = __shfl_sync(0xffffffffu, sc[0][f % NS], (lane & 28) | (h * (FB / NS) + f / NS));
+                const int m1 = __shfl_sync(0xffffffffu, sc[1][f % NS], (lane & 28) | (h * (FB / NS) + f / NS));
+                uint32_t w0[GB], w1[GB], a[GB][4];
+                const uint32_t at = wbase ^ (f * 16 * GB);
+                lds<GB>(w0, at);
+                lds<GB>(w1, at + 1024);
 #pragma unroll
                 for (int b = 0; b < GB; ++b) {
-                    const uint32_t at = wrow + (((uint32_t)(f * GB + b) ^ g7) << 4);
-                    const uint32_t w0 = lds32(at), w1 = lds32(at + 1024);
-                    a[b][0] = (w0 << 4) & 0xf0f0f0f0u;
-                    a[b][1] = (w1 << 4) & 0xf0f0f0f0u;
-                    a[b][2] = w0 & 0xf0f0f0f0u;
-                    a[b][3] = w1 & 0xf0f0f0f0u;
+                    a[b][0] = (w0[b] << 4) & 0xf0f0f0f0u;
+                    a[b][1] = (w1[b] << 4) & 0xf0f0f0f0u;
+                    a[b][2] = w0[b] & 0xf0f0f0f0u;
+                    a[b][3] = w1[b] & 0xf0f0f0f0u;
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     if (NT > 1 && n * 8 >= ntok) break;
                     int acc[LT][4];
+                    const uint32_t xb = xat + xtok[n];
 #pragma unroll
-                    for (int b = 0; b < GB; ++b) {
-                        const uint32_t xb = xblk + (f * GB + b) * cstride + n * 256;
-                        if (PACK) {
-                            uint2 v = make_uint2(0, 0);
-                            if (col_ok) v = lds64(xb);
-                            mma_s8u8(acc[0], a[b], col_top ? 0u : v.x, col_top ? 0u : v.y, b == 0);
-                            mma_s8s8(acc[0], a[b], col_top ? v.x : 0u, col_top ? v.y : 0u, false);
-                        } else {
+                    for (int l = 0; l < LT; ++l) {
+                        uint32_t x[XP::PIECES][2 * XP::MMAS];
 #pragma unroll
-                            for (int l = 0; l < L; ++l) {
-                                uint2 v = make_uint2(0, 0);
-                                if (n * 8 + g < ntok) v = lds64(xb + l * p.tb * 32);
-                                if (l < L - 1) mma_s8u8(acc[l < LT ? l : 0], a[b], v.x, v.y, b == 0);
-                                else mma_s8s8(acc[l < LT ? l : 0], a[b], v.x, v.y, b == 0);
+                        for (int q = 0; q < XP::PIECES; ++q)
+                            lds<2 * XP::MMAS>(x[q], xb + l * LIMB_STRIDE + q * PIECE_STRIDE);
+#pragma unroll
+                        for (int b = 0; b < GB; ++b) {
+                            const uint32_t x0 = x[b / XP::MMAS][2 * (b % XP::MMAS)], x1 = x[b / XP::MMAS][2 * (b % XP::MMAS) + 1];
+                            const bool keep = f == FB - 1;
+                            if (PACK) {
+                                mma_step<false>(acc[0], a[b], col_top ? 0u : x0, col_top ? 0u : x1, b == 0, keep);
+                                mma_step<true>(acc[0], a[b], col_top ? x0 : 0u, col_top ? x1 : 0u, false, keep);
+                            } else if (l < L - 1) {
+                                mma_step<false>(acc[l], a[b], x0, x1, b == 0, keep);
+                            } else {
+                                mma_step<true>(acc[l], a[b], x0, x1, b == 0, keep);
                             }
                         }
                     }
@@ -385,65 +501,62 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ CUt
                         }
                     }
                 }
+                xat += CSTRIDE;
             }
-            // The slot's words have been multiplied (the MMAs above took them), so it may be filled again.
-            if (++take == p.slots) {
-                take = 0;
-                phase ^= 1u;
-            }
-            __syncwarp();
+            // The box's words have been multiplied (the MMAs above took them: every lane's loads are done), so
+            // its slot may be filled again.
+            take = take + 1 == p.slots ? 0 : take + 1;
+            phase ^= take == 0 ? 1u : 0u;
             issue();
+            }
         }
-        // ---- partial sums of the block
-        uint64_t* const mine = part + warp * 16 * AC;
+        // ---- the round's partial sums: of wpr warps here, and of the cluster's other columns
+        if (p.once) __syncthreads();  // every box has been multiplied: the sums may take the ring's place
+        uint64_t* const mine = part + warp * 16 * PS;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-                *reinterpret_cast<ulonglong2*>(mine + (g + 8 * h) * AC + n * 8 + 2 * t) =
-                    make_ulonglong2((uint64_t)acc64[n][2 * h], (uint64_t)acc64[n][2 * h + 1]);
-        if (pending) finish_pending();
-        __syncthreads();
-        const int row_first = (u - q * p.row_rounds) * rows_round;
-        const int outs = rows_round * ntok;
-        for (int o = threadIdx.x; o < outs; o += THREADS) {
-            const int rr = o % rows_round, tok = o / rows_round;
-            uint64_t s = 0;
-            const uint64_t* from = part + ((rr >> 4) * 16 + (rr & 15)) * AC;
-            for (int w = 0; w < wpr; ++w, from += (size_t)rt * 16 * AC) {
-                if (PACK) {
-#pragma unroll
-                    for (int l = 0; l < L; ++l) s += from[l * TP + tok] << (8 * l);
-                } else {
-                    s += from[tok];
-                }
-            }
-            if (p.cs == 1) {
-                const int r = row_first + rr;
-                if (r < p.a.rows) p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)s >> (p.a.shift + 4));
-            } else {
-                const int per_rank = (rows_round * p.tb + p.cs - 1) / p.cs;
-                const uint32_t local = smem_u32(&sums[(buf * p.cs + rank) * per_rank + o / p.cs]);
-                const uint32_t to = mapa(local, (uint32_t)(o % p.cs));
-                asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to), "l"(s) : "memory");
-            }
-        }
+            for (int i = 0; i < 4; ++i) mine[(row + 8 * (i >> 1)) * PS + n * 8 + 2 * t + (i & 1)] = (uint64_t)acc64[n][i];
+        __syncwarp();
         if (p.cs > 1) {
             cluster_arrive();
-            pending = true;
-            pend_row0 = row_first;
-            pend_ntok = ntok;
-            pend_p0 = p0;
-            pend_buf = buf;
-            buf ^= 1u;
+            cluster_wait();
+        } else {
+            __syncthreads();
         }
-        __syncthreads();  // the partial sums and the activations may be overwritten
-    }
-    if (p.cs > 1) {
-        if (pending) finish_pending();
-        // no block leaves while another may still write into it
-        cluster_arrive();
-        cluster_wait();
+        const int row_first = (u - q * p.row_rounds) * rows_round;
+        const int outs = rows_round * ntok;
+        for (int o = (int)rank * THREADS + threadIdx.x; o < outs; o += p.cs * THREADS) {
+            const int tok = (int)((unsigned)o / (unsigned)rows_round), rr = o - tok * rows_round, r = row_first + rr;
+            if (r >= p.a.rows) continue;
+            uint64_t s = 0;
+            const uint32_t from = smem_u32(part + rr * PS + tok);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                if (c >= p.cs) break;
+                const uint32_t there = p.cs > 1 ? mapa(from, (uint32_t)c) : from;
+#pragma unroll 4
+                for (int w = 0; w < wpr; ++w) {
+#pragma unroll
+                    for (int l = 0; l < (PACK ? L : 1); ++l) {
+                        const uint32_t at = there + (uint32_t)((w * rows_round * PS + l * TP) * 8);
+                        uint64_t v;
+                        if (p.cs > 1) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+                        else asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
+                        s += v << (PACK ? 8 * l : 0);
+                    }
+                }
+            }
+            p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)s >> (p.a.shift + 4));
+        }
+        // the sums and the activations may be overwritten (and no block leaves while another reads from it)
+        __syncwarp();
+        if (p.cs > 1) {
+            cluster_arrive();
+            cluster_wait();
+        } else if (!p.once) {
+            __syncthreads();
+        }
     }
     if (*abort_s) __nanosleep(200000);  // let copies still in flight land
 }
@@ -453,9 +566,9 @@ struct Plan {
     int grid, smem;
 };
 
-template <int L, int NT, bool PACK, int GB>
+template <int L, int TC, int GB>
 int64_t launch(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan) {
-    auto kern = kernel<L, NT, PACK, GB>;
+    auto kern = gemv_w4_mma_kernel<L, TC, GB>;
     static thread_local int done_for = -1;
     if (done_for != ctx->device) {
         MB200_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
@@ -479,23 +592,33 @@ int64_t launch(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan) {
     MB200_CUDA(cudaLaunchKernelEx(&lc, kern, tm, plan.p));
     prof_end(ctx);
     count_launch();
-    return check_launch("gemv_w4 kernel");
+    return check_launch("gemv_w4_mma_kernel");
 }
 
-template <int L, int NT, bool PACK>
+template <int L, int TC>
 int64_t launch_gb(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan) {
     const int g32 = plan.p.group32;
-    if (g32 % 4 == 0) return launch<L, NT, PACK, 4>(ctx, tm, plan);
-    if (g32 % 2 == 0) return launch<L, NT, PACK, 2>(ctx, tm, plan);
-    return launch<L, NT, PACK, 1>(ctx, tm, plan);
+    if (g32 % 4 == 0) return launch<L, TC, 4>(ctx, tm, plan);
+    if (g32 % 2 == 0) return launch<L, TC, 2>(ctx, tm, plan);
+    return launch<L, TC, 1>(ctx, tm, plan);
+}
+
+// tc: tokens per block of the kernel, a power of two up to 32.
+template <int L>
+int64_t launch_tc(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int tc) {
+    if (tc == 1) return launch_gb<L, 1>(ctx, tm, plan);
+    if (tc == 2) return launch_gb<L, 2>(ctx, tm, plan);
+    if (tc == 4) return launch_gb<L, 4>(ctx, tm, plan);
+    if (tc == 8) return launch_gb<L, 8>(ctx, tm, plan);
+    if (tc == 16) return launch_gb<L, 16>(ctx, tm, plan);
+    return launch_gb<L, 32>(ctx, tm, plan);
 }
 
 // Clusters of `cs` blocks that the device holds at once (asked once per device).
 int cluster_fit(DeviceCtx* ctx, int cs);
-// nt: blocks of eight tokens of the kernel; 0 = packed.
-int64_t launch_i8(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int nt);
-int64_t launch_i16(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int nt);
-int64_t launch_q16(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int nt);
+int64_t launch_i8(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int tc);
+int64_t launch_i16(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int tc);
+int64_t launch_q16(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int tc);
 
 }  // namespace w4
 }  // namespace mb200

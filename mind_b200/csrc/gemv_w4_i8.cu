@@ -12,7 +12,7 @@ int cluster_fit(DeviceCtx* ctx, int cs) {
         for (int& f : fit) f = -1;
     }
     if (fit[cs] >= 0) return fit[cs];
-    auto kern = kernel<1, 1, false, 4>;
+    auto kern = gemv_w4_mma_kernel<1, 1, 4>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX);
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)(ctx->sm_count / cs * cs), 1, 1);
@@ -33,10 +33,8 @@ int cluster_fit(DeviceCtx* ctx, int cs) {
     return fit[cs] = n;
 }
 
-int64_t launch_i8(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int nt) {
-    if (nt <= 1) return launch_gb<1, 1, false>(ctx, tm, plan);
-    if (nt == 2) return launch_gb<1, 2, false>(ctx, tm, plan);
-    return launch_gb<1, 4, false>(ctx, tm, plan);
+int64_t launch_i8(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int tc) {
+    return launch_tc<1>(ctx, tm, plan, tc);
 }
 
 }  // namespace w4

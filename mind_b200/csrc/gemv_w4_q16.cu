@@ -4,11 +4,8 @@
 namespace mb200 {
 namespace w4 {
 
-int64_t launch_q16(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int nt) {
-    if (nt == 0) return launch_gb<4, 1, true>(ctx, tm, plan);
-    if (nt <= 1) return launch_gb<4, 1, false>(ctx, tm, plan);
-    if (nt == 2) return launch_gb<4, 2, false>(ctx, tm, plan);
-    return launch_gb<4, 4, false>(ctx, tm, plan);
+int64_t launch_q16(DeviceCtx* ctx, const CUtensorMap& tm, const Plan& plan, int tc) {
+    return launch_tc<4>(ctx, tm, plan, tc);
 }
 
 }  // namespace w4
