@@ -111,7 +111,8 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
             const double mem = bytes * (active / 3400.0 > 1.0 / 60.0 ? active / 3400.0 : 1.0 / 60.0);
             const double work = steps * step;
             const double round = (mem > work ? mem : work) + 0.15 * (mem > work ? work : mem) + (cs > 1 ? 2000.0 : 700.0);
-            const double cost = most * round + (double)kb_slice * w4::KB / 8 * tb / w4::THREADS * fill * 4 / 0.7;
+            // (a cluster's rounds wait for one another's remote reads: 4 us each were measured)
+            const double cost = most * round + (cs > 1 ? (most - 1) * 7000.0 : 0.0) + (double)kb_slice * w4::KB / 8 * tb / w4::THREADS * fill * 4 / 0.7;
             if (best == 0 || cost < best) {
                 best = cost;
                 w4::Params& p = out->p;

@@ -367,41 +367,49 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
             const unsigned rows_e = bound[e_now + 1] - bound[e_now], per = rows_e / nb, extra = rows_e - per * nb;
             p0 = bound[e_now] + (int)(i * per + min(i, extra));
             ntok = (int)per + (i < extra ? 1 : 0);
-            // A thread owns groups of eight columns and takes them token by token (several tokens at once where
-            // the columns are few), a batch of loads before the first store.
+            // A thread owns groups of eight columns and takes them token by token (the block several tokens at once
+            // where the columns are few): 32 registers of loads before the first store, and the first
+            // batch before the weights are asked for, behind which it would have to queue.
             const int octs = (kb_hi - kb_lo) * (KB / 8);
             const int width = octs < THREADS ? octs : THREADS, tstep = THREADS / width;
-            const int tok0 = (int)threadIdx.x / width;
-            constexpr int BATCH = L == 4 ? 4 : 8;
-            for (int o = (int)threadIdx.x - tok0 * width; o < octs && tok0 < tstep; o += width) {
-                const int m = o % GB;  // MMA that takes these eight columns
-                const uint32_t at = xs + o / (4 * GB) * CSTRIDE + (m / XP::MMAS) * PIECE_STRIDE +
-                                    (o / GB & 3) * XP::BYTES + (m % XP::MMAS) * 8;
-                const int64_t k = (int64_t)kb_lo * KB + 8 * o;
-                for (int tk = tok0; tk < ntok; tk += BATCH * tstep) {
-                    uint32_t v[BATCH][2 * L];
+            const int tok0 = (int)threadIdx.x / width, o0 = (int)threadIdx.x - tok0 * width;
+            constexpr int BATCH = 16 / L;
+            int lo = o0, lt = tok0, so = o0, st = tok0;  // next to load, next to store: columns, token
+            if (tok0 >= tstep || tok0 >= ntok) lo = so = octs;
+            while (so < octs) {
+                uint32_t v[BATCH][2 * L];
 #pragma unroll
-                    for (int b = 0; b < BATCH; ++b) {
-                        const int tok = tk + b * tstep;
+                for (int b = 0; b < BATCH; ++b) {
 #pragma unroll
-                        for (int j = 0; j < 2 * L; ++j) v[b][j] = 0;
-                        if (tok >= ntok) break;
-                        const int64_t xr = p.a.rows_of ? p.a.rows_of[p0 + tok] : p0 + tok;
-                        if (xr >= 0 && xr < p.a.x_rows) load8<L>(p, xr, k, v[b]);
+                    for (int j = 0; j < 2 * L; ++j) v[b][j] = 0;
+                    if (lo >= octs) break;
+                    const int64_t xr = p.a.rows_of ? p.a.rows_of[p0 + lt] : p0 + lt;
+                    if (xr >= 0 && xr < p.a.x_rows) load8<L>(p, xr, (int64_t)kb_lo * KB + 8 * lo, v[b]);
+                    lt += tstep;
+                    if (lt >= ntok) {
+                        lt = tok0;
+                        lo += width;
                     }
-                    if (!asked) {
-                        asked = true;
-                        for (int s = 0; s < p.slots; ++s) issue();
-                    }
+                }
+                if (!asked) {
+                    asked = true;
+                    for (int s = 0; s < p.slots; ++s) issue();
+                }
 #pragma unroll
-                    for (int b = 0; b < BATCH; ++b) {
-                        const int tok = tk + b * tstep;
-                        if (tok >= ntok) break;
+                for (int b = 0; b < BATCH; ++b) {
+                    if (so >= octs) break;
+                    const int m = so % GB;  // MMA that takes these eight columns
+                    const uint32_t at = xs + so / (4 * GB) * CSTRIDE + (m / XP::MMAS) * PIECE_STRIDE +
+                                        (st * 4 + (so / GB & 3)) * XP::BYTES + (m % XP::MMAS) * 8;
 #pragma unroll
-                        for (int l = 0; l < L; ++l)
-                            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + l * LIMB_STRIDE + tok * 4 * XP::BYTES),
-                                         "r"(limb4<L>(v[b], l, 0)), "r"(limb4<L>(v[b], l, 1))
-                                         : "memory");
+                    for (int l = 0; l < L; ++l)
+                        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(at + l * LIMB_STRIDE),
+                                     "r"(limb4<L>(v[b], l, 0)), "r"(limb4<L>(v[b], l, 1))
+                                     : "memory");
+                    st += tstep;
+                    if (st >= ntok) {
+                        st = tok0;
+                        so += width;
                     }
                 }
             }
@@ -526,28 +534,38 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         }
         const int row_first = (u - q * p.row_rounds) * rows_round;
         const int outs = rows_round * ntok;
-        for (int o = (int)rank * THREADS + threadIdx.x; o < outs; o += p.cs * THREADS) {
-            const int tok = (int)((unsigned)o / (unsigned)rows_round), rr = o - tok * rows_round, r = row_first + rr;
-            if (r >= p.a.rows) continue;
-            uint64_t s = 0;
-            const uint32_t from = smem_u32(part + rr * PS + tok);
+        const unsigned by = (unsigned)rows_round;
+        constexpr int OUTS = 4;  // outputs a thread adds up at a time: their (remote) loads travel together
+        for (int o0 = (int)rank * THREADS + threadIdx.x; o0 < outs; o0 += OUTS * p.cs * THREADS) {
+            uint64_t sum[OUTS];
+            uint32_t from[OUTS];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                if (c >= p.cs) break;
-                const uint32_t there = p.cs > 1 ? mapa(from, (uint32_t)c) : from;
-#pragma unroll 4
-                for (int w = 0; w < wpr; ++w) {
-#pragma unroll
-                    for (int l = 0; l < (PACK ? L : 1); ++l) {
-                        const uint32_t at = there + (uint32_t)((w * rows_round * PS + l * TP) * 8);
-                        uint64_t v;
-                        if (p.cs > 1) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
-                        else asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v) : "r"(at) : "memory");
-                        s += v << (PACK ? 8 * l : 0);
-                    }
-                }
+            for (int b = 0; b < OUTS; ++b) {
+                const int o = min(o0 + b * p.cs * THREADS, outs - 1), tok = (int)((unsigned)o / by);
+                sum[b] = 0;
+                from[b] = smem_u32(part + (o - tok * rows_round) * PS + tok);
             }
-            p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)s >> (p.a.shift + 4));
+            for (int c = 0; c < p.cs; ++c)
+                for (int w = 0; w < wpr; ++w) {
+                    uint64_t v[OUTS][PACK ? L : 1];
+#pragma unroll
+                    for (int b = 0; b < OUTS; ++b)
+#pragma unroll
+                        for (int l = 0; l < (PACK ? L : 1); ++l) {
+                            const uint32_t at = from[b] + (uint32_t)((w * rows_round * PS + l * TP) * 8);
+                            if (p.cs > 1) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
+                            else asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v[b][l]) : "r"(at) : "memory");
+                        }
+#pragma unroll
+                    for (int b = 0; b < OUTS; ++b)
+#pragma unroll
+                        for (int l = 0; l < (PACK ? L : 1); ++l) sum[b] += v[b][l] << (PACK ? 8 * l : 0);
+                }
+#pragma unroll
+            for (int b = 0; b < OUTS; ++b) {
+                const int o = o0 + b * p.cs * THREADS, tok = (int)((unsigned)o / by), r = row_first + o - tok * rows_round;
+                if (o < outs && r < p.a.rows) p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)sum[b] >> (p.a.shift + 4));
+            }
         }
         // the sums and the activations may be overwritten (and no block leaves while another reads from it)
         __syncwarp();
