@@ -640,13 +640,24 @@ int64_t launch_grouped_any(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a
                            bool early) {
     // (a kernel may be asked for by name: mind_b200_set_gemm_path 10 / 3 / 2)
     const int pair = tuning().pair_mode.load(), small = tuning().small_tile.load();
-    const int64_t avg = g.m / g.experts;
     if (small == 1) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
     if (pair == 2) return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb, early);
     if (pair == 1) return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb, early);
-    if (avg <= 48) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
-    if (avg < 384) return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb, early);
-    return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb, early);
+    // The host knows the rows and the experts, not how the rows are spread: tiles are counted as if every
+    // expert had the average, half of its last tile empty.
+    const double m = (double)g.m, half = g.experts / 2.0, n256 = (double)((g.n + 255) / 256);
+    const double avg = m / g.experts;
+    const double single_tiles = (m / 128 + half) * n256, pair_tiles = (m / 256 + half) * n256;
+    // 32-row tiles where the weights are most of the traffic (2048 x 2816, 64 experts: 58.5 us against 58.2 of
+    // 128-row tiles at 8 rows an expert, 70 against 63 at 16), or where the wide tiles would leave SMs idle
+    // (4096 x 1024, 8 experts: 16.4 against 21 us at 32 rows an expert).
+    if (avg <= 8 || (avg <= 48 && single_tiles < ctx->sm_count)) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
+    // Pairs of CTAs move a third less per product (32768 x 4096 x 4096: 390 us against 443), unless their
+    // coarser tiles cost a wave (4096 x 4096 x 2048, 8 experts: 42 us in three waves against 38 in two).
+    const double single_waves = single_tiles / ctx->sm_count, pair_waves = pair_tiles / (ctx->sm_count / 2);
+    const auto up = [](double w) { return w < 8 ? (double)(int64_t)(w + 0.999) : w; };
+    if (up(pair_waves) <= 1.13 * up(single_waves)) return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb, early);
+    return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb, early);
 }
 
 }  // namespace

@@ -4,11 +4,14 @@
 //   the kept i, in order of (ids[i], i), are p = 0, 1, ...:  rows[p] = i / per,  place[i] = p
 //   place[i] = -1 where ids[i] names no expert (padding)
 //
-// One cluster of 1, 2, 4 or 8 blocks, one launch.  Every warp owns a contiguous piece of the ids and a
+// Every warp owns a contiguous piece of the ids and a
 // histogram of its own in shared memory; two passes over the ids (count, then place) with a scan of the
 // histograms between them, expert-major and (block, warp)-minor, which is what makes the order stable.
-// The blocks meet in shared memory: each publishes its totals per expert and reads the others' remotely,
-// so nothing is kept in global memory and no block waits for one that may not be running.
+// Up to 16384 ids take one launch of one cluster of 1, 2, 4 or 8 blocks, which meet in shared memory: each
+// publishes its totals per expert and reads the others' remotely.  More ids take two launches of up to one
+// block per SM: the first leaves the blocks' totals in scratch, the second counts again, adds them up and
+// places (300126 ids over 160 experts: 75 us on a cluster, whose eight SMs are bound by their scattered
+// stores).  Either way no block waits for one that may not be running.
 //
 // Inside 32 ids the rank of a lane among the lanes of the same expert is a population count of
 // __match_any_sync's mask, so no atomics are used and the result does not depend on timing.
@@ -23,15 +26,26 @@ namespace {
 
 constexpr int MAX_CLUSTER = 8;
 
+// Expert e's count over the warps (a multiple of four), four loads at a time.
+__device__ __forceinline__ int32_t column(const int32_t* hist, int warps, int experts, int e) {
+    int32_t n[4] = {0, 0, 0, 0};
+    for (int w = 0; w < warps; w += 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) n[j] += hist[(w + j) * experts + e];
+    return n[0] + n[1] + n[2] + n[3];
+}
+
 // Shared memory: hist[warps][experts], then (clusters) total[experts].
 __global__ void __launch_bounds__(1024)
 expert_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ offsets, int32_t* __restrict__ rows,
-                   int32_t* __restrict__ place, int64_t count, int experts, unsigned per, int blocks) {
+                   int32_t* __restrict__ place, int64_t count, int experts, unsigned per, int blocks, int phase,
+                   int32_t* __restrict__ totals) {  // phase 0: a cluster does it all; 1: count; 2: place
     extern __shared__ int32_t hist[];
     __shared__ int32_t warp_sum[32];
     __shared__ int32_t carry;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const int block = blockIdx.x;  // the grid is one cluster
+    const int block = blockIdx.x;
+    const bool cluster = phase == 0 && blocks > 1;  // the grid is one cluster
     int32_t* const total = hist + warps * experts;
     griddep_launch_dependents();
     for (int i = threadIdx.x; i < warps * experts; i += blockDim.x) hist[i] = 0;
@@ -62,11 +76,15 @@ expert_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ offset
         }
     }
     __syncthreads();
-    if (blocks > 1) {  // publish this block's totals
+    if (phase == 1) {
         for (int e = threadIdx.x; e < experts; e += blockDim.x) {
-            int32_t n = 0;
-            for (int w = 0; w < warps; ++w) n += hist[w * experts + e];
-            total[e] = n;
+            totals[block * experts + e] = column(hist, warps, experts, e);
+        }
+        return;
+    }
+    if (cluster) {  // publish this block's totals
+        for (int e = threadIdx.x; e < experts; e += blockDim.x) {
+            total[e] = column(hist, warps, experts, e);
         }
         cluster_arrive();
         cluster_wait();
@@ -77,7 +95,14 @@ expert_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ offset
         const int e = e0 + threadIdx.x;
         int32_t all = 0, before_me = 0;  // of this expert: everywhere, and in the blocks before this one
         if (e < experts) {
-            if (blocks > 1) {
+            if (phase == 2) {
+#pragma unroll 8
+                for (int b = 0; b < blocks; ++b) {
+                    const int32_t n = totals[b * experts + e];
+                    all += n;
+                    before_me += b < block ? n : 0;
+                }
+            } else if (cluster) {
                 int32_t n[MAX_CLUSTER];
                 const uint32_t at = smem_u32(total + e);
 #pragma unroll
@@ -91,7 +116,7 @@ expert_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ offset
                     before_me += b < block ? n[b] : 0;
                 }
             } else {
-                for (int w = 0; w < warps; ++w) all += hist[w * experts + e];
+                all = column(hist, warps, experts, e);
             }
         }
         int32_t incl = all;
@@ -107,10 +132,15 @@ expert_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ offset
             int32_t at = before + incl - all;
             if (block == 0) offsets[e] = at;
             at += before_me;
-            for (int w = 0; w < warps; ++w) {
-                const int32_t n = hist[w * experts + e];
-                hist[w * experts + e] = at;
-                at += n;
+            for (int w = 0; w < warps; w += 4) {
+                int32_t n[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) n[j] = hist[(w + j) * experts + e];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    hist[(w + j) * experts + e] = at;
+                    at += n[j];
+                }
             }
         }
         __syncthreads();
@@ -144,7 +174,7 @@ expert_plan_kernel(const int32_t* __restrict__ ids, int32_t* __restrict__ offset
             }
         }
     }
-    if (blocks > 1) {  // no block leaves while another may still read its totals
+    if (cluster) {  // no block leaves while another may still read its totals
         __syncwarp();
         cluster_arrive();
         cluster_wait();
@@ -161,8 +191,19 @@ int64_t launch_expert_plan(DeviceCtx* ctx, const int32_t* ids, int32_t* offsets,
     while (warps > 4 && (size_t)warps * experts * 4 > (size_t)128 << 10) warps >>= 1;
     const int64_t groups = (count + 31) / 32;
     while (warps > 4 && warps / 2 >= groups) warps >>= 1;
+    // blocks of the two-launch form: as many as keep the table of totals, which every block reads, small
+    int64_t wide = 80000 / experts;
+    if (wide > ctx->sm_count) wide = ctx->sm_count;
+    const bool two = count > 16384 && wide > 2 * MAX_CLUSTER;
     int blocks = 1;
-    while (blocks < MAX_CLUSTER && groups > (int64_t)4 * warps * blocks) blocks *= 2;
+    while (!two && blocks < MAX_CLUSTER && groups > (int64_t)4 * warps * blocks) blocks *= 2;
+    int32_t* totals = nullptr;
+    if (two) {
+        warps = warps < 16 ? warps : 16;
+        blocks = (int)(wide < groups / warps ? wide : groups / warps);
+        MB200_TRY(arena_reserve(ctx, ctx->scratch, (size_t)blocks * experts * 4 + 2048));
+        totals = static_cast<int32_t*>(arena_take(ctx->scratch, (size_t)blocks * experts * 4));
+    }
     const size_t smem = (size_t)(warps + 1) * experts * 4;
     static thread_local int done_for = -1;
     if (done_for != ctx->device) {
@@ -182,10 +223,14 @@ int64_t launch_expert_plan(DeviceCtx* ctx, const int32_t* ids, int32_t* offsets,
     at[1].val.clusterDim.y = 1;
     at[1].val.clusterDim.z = 1;
     lc.attrs = at;
-    lc.numAttrs = blocks > 1 ? 2 : 1;
+    lc.numAttrs = !two && blocks > 1 ? 2 : 1;
+    const unsigned div = (unsigned)(per < 0x7fffffff ? per : 0x7fffffff);
     prof_begin(ctx);
-    MB200_CUDA(cudaLaunchKernelEx(&lc, expert_plan_kernel, ids, offsets, rows, place, count, (int)experts,
-                                  (unsigned)(per < 0x7fffffff ? per : 0x7fffffff), blocks));
+    if (two) {
+        MB200_CUDA(cudaLaunchKernelEx(&lc, expert_plan_kernel, ids, offsets, rows, place, count, (int)experts, div, blocks, 1, totals));
+        count_launch();
+    }
+    MB200_CUDA(cudaLaunchKernelEx(&lc, expert_plan_kernel, ids, offsets, rows, place, count, (int)experts, div, blocks, two ? 2 : 0, totals));
     prof_end(ctx);
     count_launch();
     return check_launch("expert_plan_kernel");
