@@ -74,7 +74,7 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
     const int kb_total = (int)((a.cols + w4::KB - 1) / w4::KB);
     const int g32 = (int)(a.group / 32 % 4), gb = g32 == 0 ? 4 : (g32 == 2 ? 2 : 1);
     const size_t table = align_up((size_t)(a.experts + 1) * 8, 128);
-    const size_t part = align_up((size_t)w4::WARPS * 16 * (ac + 1) * 8, 1024);
+    const size_t part = align_up((size_t)w4::WARPS * ac * 17 * 8, 1024);
     // Instructions of a warp per unit, and the clocks of a unit that nothing overlaps
     const double mmas = pack ? 2.0 : (double)L * tok8;                                     // per 32 columns
     const double per32 = 8.0 + mmas + (pack ? 1.0 : mmas) * (gb == 1 ? 1.0 : 0.5) + (pack ? 4.0 : 0.0);

@@ -101,27 +101,29 @@ struct XPiece {
     static constexpr int BYTES = GB == 1 ? 8 : 16, PIECES = 8 * GB / BYTES, MMAS = BYTES / 8;
 };
 
-// Eight activations k .. k + 7 of row xr as they lie in memory, 2 * L words (zeros past the end).
+// Eight activations from element `at` on, as they lie in memory: 2 * L words, aligned.
+template <int L>
+__device__ __forceinline__ void load8_vec(const void* x, int64_t at, uint32_t (&v)[2 * L]) {
+    const char* const p = static_cast<const char*>(x) + at * L;
+    if constexpr (L == 1) {
+        const uint2 w = *reinterpret_cast<const uint2*>(p);
+        v[0] = w.x;
+        v[1] = w.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < L / 2; ++i) {
+            const uint4 w = *reinterpret_cast<const uint4*>(p + 16 * i);
+            v[4 * i] = w.x;
+            v[4 * i + 1] = w.y;
+            v[4 * i + 2] = w.z;
+            v[4 * i + 3] = w.w;
+        }
+    }
+}
+// The same of row xr from column k on, at any alignment, with zeros past the end.
 template <int L>
 __device__ __forceinline__ void load8(const Params& p, int64_t xr, int64_t k, uint32_t (&v)[2 * L]) {
     const char* const at = static_cast<const char*>(p.a.x) + (xr * p.a.cols + k) * L;
-    if (p.x_vec && k + 8 <= p.a.cols) {
-        if constexpr (L == 1) {
-            const uint2 w = *reinterpret_cast<const uint2*>(at);
-            v[0] = w.x;
-            v[1] = w.y;
-        } else {
-#pragma unroll
-            for (int i = 0; i < L / 2; ++i) {
-                const uint4 w = *reinterpret_cast<const uint4*>(at + 16 * i);
-                v[4 * i] = w.x;
-                v[4 * i + 1] = w.y;
-                v[4 * i + 2] = w.z;
-                v[4 * i + 3] = w.w;
-            }
-        }
-        return;
-    }
 #pragma unroll
     for (int i = 0; i < 2 * L; ++i) v[i] = 0;
 #pragma unroll
@@ -159,7 +161,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
     constexpr int NT = (TC + 7) / 8;      // blocks of eight tokens
     constexpr int LT = PACK ? 1 : L;      // accumulator sets between scalings
     constexpr int AC = 8 * NT;            // accumulator columns of a warp
-    constexpr int PS = AC + 1;            // stride of a row of partial sums: rows side by side hit different banks
+    constexpr int PS = 17;                // partial sums: a column's 16 rows lie side by side, so that remote reads are whole lines
     constexpr int TP = PACK ? 8 / L : 1;  // tokens per limb in a packed set
     constexpr int NF = KB / 32 / GB;      // scalings per unit
     constexpr int FB = NF / 2;            // per box
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
     const uint32_t ring0 = base + HEAD_BYTES;
     int* const misc = reinterpret_cast<int*>(gbase + WARPS * MAX_SLOTS * 8);
     volatile int* const abort_s = misc;
-    uint64_t* const part = reinterpret_cast<uint64_t*>(gbase + p.off_part);  // [warp][16][PS]
+    uint64_t* const part = reinterpret_cast<uint64_t*>(gbase + p.off_part);  // [warp][AC][PS]
     const uint32_t xs = base + p.off_x;
     int* const bound = reinterpret_cast<int*>(gbase + p.off_table);  // [experts + 1] first row of each
     int* const cumb = bound + p.a.experts + 1;                       // [experts + 1] token blocks before each
@@ -368,30 +370,54 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
             p0 = bound[e_now] + (int)(i * per + min(i, extra));
             ntok = (int)per + (i < extra ? 1 : 0);
             // A thread owns groups of eight columns and takes them token by token (the block several tokens at once
-            // where the columns are few): 32 registers of loads before the first store, and the first
-            // batch before the weights are asked for, behind which it would have to queue.
+            // where the columns are few): 32 registers of loads before the first store, and
+            // all of them before the weights are asked for, behind which they would have to queue.
             const int octs = (kb_hi - kb_lo) * (KB / 8);
             const int width = octs < THREADS ? octs : THREADS, tstep = THREADS / width;
             const int tok0 = (int)threadIdx.x / width, o0 = (int)threadIdx.x - tok0 * width;
-            constexpr int BATCH = 16 / L;
+            constexpr int BATCH = TC <= 2 ? 2 * TC : 16 / L;
             int lo = o0, lt = tok0, so = o0, st = tok0;  // next to load, next to store: columns, token
             if (tok0 >= tstep || tok0 >= ntok) lo = so = octs;
             while (so < octs) {
                 uint32_t v[BATCH][2 * L];
+                if (p.x_vec) {
+                    // No branch between the loads, which would end one before the next begins: what is not there is
+                    // read from the first row and replaced by zeros.
+                    int64_t at[BATCH];
+                    unsigned there = 0;
 #pragma unroll
-                for (int b = 0; b < BATCH; ++b) {
+                    for (int b = 0; b < BATCH; ++b) {
+                        const int tok = min(lt, ntok - 1);
+                        const int64_t xr = p.a.rows_of ? p.a.rows_of[p0 + tok] : p0 + tok, k = (int64_t)kb_lo * KB + 8 * lo;
+                        const bool ok = lo < octs && k < p.a.cols && xr >= 0 && xr < p.a.x_rows;
+                        at[b] = ok ? xr * p.a.cols + k : 0;
+                        there |= ok ? 1u << b : 0u;
+                        lt += tstep;
+                        lo += lt >= ntok ? width : 0;
+                        lt = lt >= ntok ? tok0 : lt;
+                    }
 #pragma unroll
-                    for (int j = 0; j < 2 * L; ++j) v[b][j] = 0;
-                    if (lo >= octs) break;
-                    const int64_t xr = p.a.rows_of ? p.a.rows_of[p0 + lt] : p0 + lt;
-                    if (xr >= 0 && xr < p.a.x_rows) load8<L>(p, xr, (int64_t)kb_lo * KB + 8 * lo, v[b]);
-                    lt += tstep;
-                    if (lt >= ntok) {
-                        lt = tok0;
-                        lo += width;
+                    for (int b = 0; b < BATCH; ++b) load8_vec<L>(p.a.x, at[b], v[b]);
+#pragma unroll
+                    for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+                        for (int j = 0; j < 2 * L; ++j) v[b][j] = there >> b & 1u ? v[b][j] : 0u;
+                } else {
+#pragma unroll
+                    for (int b = 0; b < BATCH; ++b) {
+#pragma unroll
+                        for (int j = 0; j < 2 * L; ++j) v[b][j] = 0;
+                        if (lo >= octs) continue;
+                        const int64_t xr = p.a.rows_of ? p.a.rows_of[p0 + lt] : p0 + lt;
+                        if (xr >= 0 && xr < p.a.x_rows) load8<L>(p, xr, (int64_t)kb_lo * KB + 8 * lo, v[b]);
+                        lt += tstep;
+                        if (lt >= ntok) {
+                            lt = tok0;
+                            lo += width;
+                        }
                     }
                 }
-                if (!asked) {
+                if (!asked && lo >= octs) {
                     asked = true;
                     for (int s = 0; s < p.slots; ++s) issue();
                 }
@@ -476,18 +502,20 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
                     if (NT > 1 && n * 8 >= ntok) break;
                     int acc[LT][4];
                     const uint32_t xb = xat + xtok[n];
+                    uint32_t x[LT][XP::PIECES][2 * XP::MMAS];
 #pragma unroll
-                    for (int l = 0; l < LT; ++l) {
-                        uint32_t x[XP::PIECES][2 * XP::MMAS];
+                    for (int l = 0; l < LT; ++l)
 #pragma unroll
-                        for (int q = 0; q < XP::PIECES; ++q)
-                            lds<2 * XP::MMAS>(x[q], xb + l * LIMB_STRIDE + q * PIECE_STRIDE);
+                        for (int q = 0; q < XP::PIECES; ++q) lds<2 * XP::MMAS>(x[l][q], xb + l * LIMB_STRIDE + q * PIECE_STRIDE);
+                    // one word of every limb's chain after the other: LT sums that do not wait for each other
 #pragma unroll
-                        for (int b = 0; b < GB; ++b) {
-                            const uint32_t x0 = x[b / XP::MMAS][2 * (b % XP::MMAS)], x1 = x[b / XP::MMAS][2 * (b % XP::MMAS) + 1];
-                            const bool keep = f == FB - 1;
-                            if (PACK) {
-                                mma_step<false>(acc[0], a[b], col_top ? 0u : x0, col_top ? 0u : x1, b == 0, keep);
+                    for (int b = 0; b < GB; ++b)
+#pragma unroll
+                        for (int l = 0; l < LT; ++l) {
+                            const uint32_t x0 = x[l][b / XP::MMAS][2 * (b % XP::MMAS)], x1 = x[l][b / XP::MMAS][2 * (b % XP::MMAS) + 1];
+                            const bool keep = f == FB - 1 && b == GB - 1 && l == LT - 1;
+                            if (PACK) {  // the unsigned columns, then the signed ones
+                                mma_step<false>(acc[0], a[b], col_top ? 0u : x0, col_top ? 0u : x1, b == 0, false);
                                 mma_step<true>(acc[0], a[b], col_top ? x0 : 0u, col_top ? x1 : 0u, false, keep);
                             } else if (l < L - 1) {
                                 mma_step<false>(acc[l], a[b], x0, x1, b == 0, keep);
@@ -495,7 +523,6 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
                                 mma_step<true>(acc[l], a[b], x0, x1, b == 0, keep);
                             }
                         }
-                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const int m = i < 2 ? m0 : m1;
@@ -520,11 +547,11 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         }
         // ---- the round's partial sums: of wpr warps here, and of the cluster's other columns
         if (p.once) __syncthreads();  // every box has been multiplied: the sums may take the ring's place
-        uint64_t* const mine = part + warp * 16 * PS;
+        uint64_t* const mine = part + warp * AC * PS;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mine[(row + 8 * (i >> 1)) * PS + n * 8 + 2 * t + (i & 1)] = (uint64_t)acc64[n][i];
+            for (int i = 0; i < 4; ++i) mine[(n * 8 + 2 * t + (i & 1)) * PS + row + 8 * (i >> 1)] = (uint64_t)acc64[n][i];
         __syncwarp();
         if (p.cs > 1) {
             cluster_arrive();
@@ -535,7 +562,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         const int row_first = (u - q * p.row_rounds) * rows_round;
         const int outs = rows_round * ntok;
         const unsigned by = (unsigned)rows_round;
-        constexpr int OUTS = 4;  // outputs a thread adds up at a time: their (remote) loads travel together
+        constexpr int OUTS = 8;  // outputs a thread adds up at a time: their (remote) loads travel together
         for (int o0 = (int)rank * THREADS + threadIdx.x; o0 < outs; o0 += OUTS * p.cs * THREADS) {
             uint64_t sum[OUTS];
             uint32_t from[OUTS];
@@ -543,7 +570,8 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
             for (int b = 0; b < OUTS; ++b) {
                 const int o = min(o0 + b * p.cs * THREADS, outs - 1), tok = (int)((unsigned)o / by);
                 sum[b] = 0;
-                from[b] = smem_u32(part + (o - tok * rows_round) * PS + tok);
+                const int rr = o - tok * rows_round;
+                from[b] = smem_u32(part + ((rr >> 4) * AC + tok) * PS + (rr & 15));
             }
             for (int c = 0; c < p.cs; ++c)
                 for (int w = 0; w < wpr; ++w) {
@@ -552,9 +580,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
                     for (int b = 0; b < OUTS; ++b)
 #pragma unroll
                         for (int l = 0; l < (PACK ? L : 1); ++l) {
-                            const uint32_t at = from[b] + (uint32_t)((w * rows_round * PS + l * TP) * 8);
-                            if (p.cs > 1) asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
-                            else asm volatile("ld.shared.u64 %0, [%1];" : "=l"(v[b][l]) : "r"(at) : "memory");
+                            const uint32_t at = from[b] + (uint32_t)((w * rt * AC + l * TP) * PS * 8);
+                            // (a block's own shared memory is part of its cluster's: rank 0 of one)
+                            asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
                         }
 #pragma unroll
                     for (int b = 0; b < OUTS; ++b)
