@@ -31,6 +31,12 @@
 
 #define MIND_B200_NATIVE_NO_LIBRARY (-3)
 
+typedef int64_t (*fn13_t)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
+                          int64_t, int64_t, int64_t);
+typedef int64_t (*fn12_t)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
+                          int64_t, int64_t);
+typedef int64_t (*fn9_t)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
+typedef int64_t (*fn7_t)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
 typedef int64_t (*fn6_t)(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t);
 typedef int64_t (*fn5_t)(int64_t, int64_t, int64_t, int64_t, int64_t);
 typedef int64_t (*fn3_t)(int64_t, int64_t, int64_t);
@@ -41,6 +47,10 @@ static struct {
     fn6_t mm_i8, mm_i8_mt, mm_q16, mm_q16_mt, mm_i16;
     fn5_t gemv_q16_mt, rmajor_q16, rmajor_i16;
     fn3_t dot_q16, dot_l1_q16, dot_i16;
+    fn13_t w4_grouped_i8, w4_grouped_i16, w4_grouped_q16;
+    fn12_t mm_grouped_i8, mm_grouped_i8_bt;
+    fn9_t w4_i8, w4_i16, w4_q16;
+    fn7_t expert_plan;
     err_t last_error;
     char load_error[512];
 } g_b200;
@@ -74,6 +84,15 @@ static void b200_load(void) {
     g_b200.dot_q16 = (fn3_t)b200_sym("__mind_blas_dot_q16_v");
     g_b200.dot_l1_q16 = (fn3_t)b200_sym("__mind_blas_dot_l1_q16_v");
     g_b200.dot_i16 = (fn3_t)b200_sym("__mind_blas_dot_i16_v");
+    g_b200.w4_i8 = (fn9_t)b200_sym("__mind_b200_gemv_w4_i8");
+    g_b200.w4_i16 = (fn9_t)b200_sym("__mind_b200_gemv_w4_i16");
+    g_b200.w4_q16 = (fn9_t)b200_sym("__mind_b200_gemv_w4_q16");
+    g_b200.w4_grouped_i8 = (fn13_t)b200_sym("__mind_b200_gemv_w4_grouped_i8");
+    g_b200.w4_grouped_i16 = (fn13_t)b200_sym("__mind_b200_gemv_w4_grouped_i16");
+    g_b200.w4_grouped_q16 = (fn13_t)b200_sym("__mind_b200_gemv_w4_grouped_q16");
+    g_b200.mm_grouped_i8 = (fn12_t)b200_sym("__mind_b200_matmul_grouped_i8");
+    g_b200.mm_grouped_i8_bt = (fn12_t)b200_sym("__mind_b200_matmul_grouped_i8_bt");
+    g_b200.expert_plan = (fn7_t)b200_sym("__mind_b200_expert_plan");
     g_b200.last_error = (err_t)b200_sym("mind_b200_last_error");
 }
 
@@ -117,3 +136,34 @@ FORWARD5(__mind_blas_matmul_rmajor_i16_v, rmajor_i16)
 FORWARD3(__mind_blas_dot_q16_v, dot_q16)
 FORWARD3(__mind_blas_dot_l1_q16_v, dot_l1_q16)
 FORWARD3(__mind_blas_dot_i16_v, dot_i16)
+
+/* products of quantised language models: no counterpart in the reference (new names) */
+#define FORWARD13(name, slot)                                                                                        \
+    int64_t name(int64_t w, int64_t s, int64_t x, int64_t r, int64_t o, int64_t y, int64_t m, int64_t rows,           \
+                 int64_t cols, int64_t group, int64_t shift, int64_t experts, int64_t x_rows) {                      \
+        return b200_ready() ? g_b200.slot(w, s, x, r, o, y, m, rows, cols, group, shift, experts, x_rows)            \
+                            : MIND_B200_NATIVE_NO_LIBRARY;                                                           \
+    }
+#define FORWARD12(name, slot)                                                                                        \
+    int64_t name(int64_t a, int64_t r, int64_t b, int64_t o, int64_t s, int64_t c, int64_t m, int64_t k, int64_t n,   \
+                 int64_t experts, int64_t a_rows, int64_t shift) {                                                   \
+        return b200_ready() ? g_b200.slot(a, r, b, o, s, c, m, k, n, experts, a_rows, shift)                         \
+                            : MIND_B200_NATIVE_NO_LIBRARY;                                                           \
+    }
+#define FORWARD9(name, slot)                                                                                         \
+    int64_t name(int64_t w, int64_t s, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols,              \
+                 int64_t group, int64_t shift) {                                                                     \
+        return b200_ready() ? g_b200.slot(w, s, x, y, tokens, rows, cols, group, shift) : MIND_B200_NATIVE_NO_LIBRARY; \
+    }
+FORWARD9(__mind_b200_gemv_w4_i8, w4_i8)
+FORWARD9(__mind_b200_gemv_w4_i16, w4_i16)
+FORWARD9(__mind_b200_gemv_w4_q16, w4_q16)
+FORWARD13(__mind_b200_gemv_w4_grouped_i8, w4_grouped_i8)
+FORWARD13(__mind_b200_gemv_w4_grouped_i16, w4_grouped_i16)
+FORWARD13(__mind_b200_gemv_w4_grouped_q16, w4_grouped_q16)
+FORWARD12(__mind_b200_matmul_grouped_i8, mm_grouped_i8)
+FORWARD12(__mind_b200_matmul_grouped_i8_bt, mm_grouped_i8_bt)
+int64_t __mind_b200_expert_plan(int64_t ids, int64_t offsets, int64_t rows, int64_t place, int64_t count, int64_t experts,
+                                int64_t per) {
+    return b200_ready() ? g_b200.expert_plan(ids, offsets, rows, place, count, experts, per) : MIND_B200_NATIVE_NO_LIBRARY;
+}

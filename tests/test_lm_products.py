@@ -2,6 +2,9 @@
 expert, and the plan that groups slots by expert.  Everything is integer arithmetic with one right
 answer, so every comparison is for equality with numpy's int64 (tolerance zero: each output is the
 exact sum, or its low 64 bits, shifted and truncated once)."""
+import os
+import subprocess
+import sys
 import threading
 
 import numpy as np
@@ -194,6 +197,40 @@ def test_no_gpu_means_a_clean_refusal():
     refused(mind_b200.ERR_NO_DEVICE, blas.gemv_w4_q16, W, S, X, Y, 1, 1, 32, 32, 0)
     refused(mind_b200.ERR_NO_DEVICE, blas.matmul_grouped_i8, W, 0, W, OFF, 0, Y, 2, 4, 4, 2, 2)
     refused(mind_b200.ERR_NO_DEVICE, blas.expert_plan, X, Y, X, Y, 4, 4, 1)
+
+
+SHIM_CHILD = r"""
+import ctypes as C, sys
+import numpy as np
+L = C.CDLL(sys.argv[1])
+i64 = C.c_int64
+def fn(name, n):
+    f = getattr(L, name); f.argtypes, f.restype = [i64] * n, i64
+    return f
+L.mind_b200_native_last_error.restype = C.c_char_p
+a = np.zeros(64, np.int32); p = a.ctypes.data
+names = {9: ["gemv_w4_i8", "gemv_w4_i16", "gemv_w4_q16"], 7: ["expert_plan"], 12: ["matmul_grouped_i8", "matmul_grouped_i8_bt"],
+         13: ["gemv_w4_grouped_i8", "gemv_w4_grouped_i16", "gemv_w4_grouped_q16"]}
+args = {9: (p, p, p, p, 1, 1, 32, 32, 99), 7: (p, p, p, p, -1, 4, 1), 12: (p, 0, p, p, 0, p, 2, 4, 4, 2, 2, 99),
+        13: (p, p, p, 0, p, p, 2, 1, 32, 32, 99, 2, 2)}
+for n, group in names.items():
+    for name in group:
+        assert fn("__mind_b200_" + name, n)(*args[n]) == int(sys.argv[2]), name
+print("ok")
+"""
+
+
+@pytest.mark.parametrize("library,status", [(mind_b200.LIB_PATH, -1), ("/nonexistent/libmind_b200.so", -3)],
+                         ids=["forwards", "missing"])
+def test_native_sources_file_forwards(tmp_path, library, status):
+    """integration/mind_b200_native.c resolves the new names too, and hands on the library's own checks."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    shim = str(tmp_path / "libshim.so")
+    subprocess.run(["gcc", "-O2", "-Wall", "-Wextra", "-Werror", "-fPIC", "-shared", "-o", shim,
+                    os.path.join(root, "integration", "mind_b200_native.c"), "-ldl", "-lpthread"], check=True)
+    r = subprocess.run([sys.executable, "-c", SHIM_CHILD, shim, str(status)], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, MIND_B200_LIB=library))
+    assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
 
 
 # ------------------------------------------------------------------------------- on a GPU
