@@ -93,7 +93,7 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
         for (int rt = 1; rt <= w4::WARPS; ++rt) {
             const int wpr = w4::WARPS / rt, steps = (kb_slice + wpr - 1) / wpr;
             const int64_t row_rounds = (tiles + rt - 1) / rt, rounds = blocks * row_rounds;
-            if (rounds > 0x3fffffff) continue;
+            if (rounds > 0x1fffffff) continue;  // (the kernel counts them, at most twice as many, in 32 bits)
             const int64_t clusters = rounds < fit ? rounds : fit;
             const int64_t most = (rounds + clusters - 1) / clusters;  // rounds of the busiest cluster
             const bool once = most == 1 && !a.offsets;
@@ -136,6 +136,49 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
     return best != 0;
 }
 
+// Tokens per block: all of them up to 32, in blocks of equal size beyond; of grouped rows the kernel
+// learns the groups' sizes itself, and twice the average leaves few experts with a second block.  The
+// choice is a pure function of the sizes, so the last few are kept per thread (it costs as much as a launch).
+bool plan_for(DeviceCtx* ctx, const W4Args& a, w4::Plan* plan, int* tc) {
+    struct Entry {
+        int64_t m, rows, cols, group, experts;
+        int kind, grouped, device, tc;
+        w4::Plan plan;
+    };
+    static thread_local Entry cache[8];
+    static thread_local int used = 0, next = 0;
+    const int grouped = a.offsets ? 1 : 0;
+    for (int i = 0; i < used; ++i) {
+        const Entry& e = cache[i];
+        if (e.m == a.m && e.rows == a.rows && e.cols == a.cols && e.group == a.group && e.experts == a.experts &&
+            e.kind == a.kind && e.grouped == grouped && e.device == ctx->device) {
+            *plan = e.plan;
+            *tc = e.tc;
+            return e.tc != 0;
+        }
+    }
+    int64_t want = a.m;
+    if (grouped) {
+        const int64_t twice = 2 * ((a.m + a.experts - 1) / a.experts) + 2;
+        if (want > twice) want = twice;
+    }
+    *tc = 0;
+    for (int64_t passes = (want + 31) / 32;; ++passes) {  // more blocks where the activations of one would not fit
+        const int tb = (int)((want + passes - 1) / passes);
+        int t = 1;
+        while (t < tb) t *= 2;
+        if (make_plan(ctx, a, tb, t, plan)) {
+            *tc = t;
+            break;
+        }
+        if (tb == 1) break;
+    }
+    cache[next] = Entry{a.m, a.rows, a.cols, a.group, a.experts, a.kind, grouped, ctx->device, *tc, *plan};
+    next = (next + 1) % 8;
+    if (used < 8) ++used;
+    return *tc != 0;
+}
+
 int64_t launch_warp_kernel(DeviceCtx* ctx, const W4Args& a) {
     int64_t blocks = (a.m * a.rows + 7) / 8;
     if (blocks > (int64_t)ctx->sm_count * 64) blocks = (int64_t)ctx->sm_count * 64;
@@ -156,22 +199,9 @@ int64_t launch_warp_kernel(DeviceCtx* ctx, const W4Args& a) {
 int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
     if (tuning().gemm_path.load() == 1 || a.cols == 0 || a.x_rows == 0) return launch_warp_kernel(ctx, a);
     const int L = a.kind == 0 ? 1 : (a.kind == 1 ? 2 : 4);
-    // Tokens per block: all of them up to 32, in blocks of equal size beyond.  Of grouped rows the kernel
-    // learns the groups' sizes itself; twice the average leaves few experts with a second block.
-    int64_t want = a.m;
-    if (a.offsets) {
-        const int64_t twice = 2 * ((a.m + a.experts - 1) / a.experts) + 2;
-        if (want > twice) want = twice;
-    }
-    int64_t passes = (want + 31) / 32;
     w4::Plan plan;
-    int tc = 1;
-    for (;; ++passes) {  // more blocks where the activations of one would not fit
-        const int tb = (int)((want + passes - 1) / passes);
-        for (tc = 1; tc < tb;) tc *= 2;
-        if (make_plan(ctx, a, tb, tc, &plan)) break;
-        if (tb == 1) return launch_warp_kernel(ctx, a);  // a row of activations too long for eight blocks
-    }
+    int tc = 0;
+    if (!plan_for(ctx, a, &plan, &tc)) return launch_warp_kernel(ctx, a);  // a row of activations too long for eight blocks
     // TMA reads rows whose pitch and base are multiples of 16 bytes; others are copied to padded rows first
     const int64_t bytes = (a.cols + 1) / 2, pitch = (int64_t)align_up((size_t)bytes, 16);
     const int8_t* w = a.w;
