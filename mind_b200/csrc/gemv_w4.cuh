@@ -84,6 +84,10 @@ __device__ __forceinline__ void mma_step(int (&d)[4], const uint32_t (&a)[4], ui
     else if (keep) mma<SIGNED, false, true>(d, a, b0, b1);
     else mma<SIGNED, false, false>(d, a, b0, b1);
 }
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
 // 4 * N bytes of shared memory.
 template <int N>
 __device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t addr) {
@@ -562,39 +566,48 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         const int row_first = (u - q * p.row_rounds) * rows_round;
         const int outs = rows_round * ntok;
         const unsigned by = (unsigned)rows_round;
-        constexpr int OUTS = 8;  // outputs a thread adds up at a time: their (remote) loads travel together
-        for (int o0 = (int)rank * THREADS + threadIdx.x; o0 < outs; o0 += OUTS * p.cs * THREADS) {
-            uint64_t sum[OUTS];
-            uint32_t from[OUTS];
+        // A thread adds up OUTS outputs at a time, the partial sums of WS warps in each, so that enough (remote)
+        // loads travel together: few outputs and many warps, or the other way round.
+        auto add_up = [&](auto outs_at_a_time, auto warps_at_a_time) {
+            constexpr int OUTS = decltype(outs_at_a_time)::value, WS = decltype(warps_at_a_time)::value, LS = PACK ? L : 1;
+            for (int o0 = (int)rank * THREADS + threadIdx.x; o0 < outs; o0 += OUTS * p.cs * THREADS) {
+                uint64_t sum[OUTS];
+                uint32_t from[OUTS];
 #pragma unroll
-            for (int b = 0; b < OUTS; ++b) {
-                const int o = min(o0 + b * p.cs * THREADS, outs - 1), tok = (int)((unsigned)o / by);
-                sum[b] = 0;
-                const int rr = o - tok * rows_round;
-                from[b] = smem_u32(part + ((rr >> 4) * AC + tok) * PS + (rr & 15));
-            }
-            for (int c = 0; c < p.cs; ++c)
-                for (int w = 0; w < wpr; ++w) {
-                    uint64_t v[OUTS][PACK ? L : 1];
-#pragma unroll
-                    for (int b = 0; b < OUTS; ++b)
-#pragma unroll
-                        for (int l = 0; l < (PACK ? L : 1); ++l) {
-                            const uint32_t at = from[b] + (uint32_t)((w * rt * AC + l * TP) * PS * 8);
-                            // (a block's own shared memory is part of its cluster's: rank 0 of one)
-                            asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
-                        }
-#pragma unroll
-                    for (int b = 0; b < OUTS; ++b)
-#pragma unroll
-                        for (int l = 0; l < (PACK ? L : 1); ++l) sum[b] += v[b][l] << (PACK ? 8 * l : 0);
+                for (int b = 0; b < OUTS; ++b) {
+                    const int o = min(o0 + b * p.cs * THREADS, outs - 1), tok = (int)((unsigned)o / by), rr = o - tok * rows_round;
+                    sum[b] = 0;
+                    from[b] = smem_u32(part + ((rr >> 4) * AC + tok) * PS + (rr & 15));
                 }
+                for (int c = 0; c < p.cs; ++c)
+                    for (int w0 = 0; w0 < wpr; w0 += WS) {
+                        uint64_t v[OUTS][WS][LS];
 #pragma unroll
-            for (int b = 0; b < OUTS; ++b) {
-                const int o = o0 + b * p.cs * THREADS, tok = (int)((unsigned)o / by), r = row_first + o - tok * rows_round;
-                if (o < outs && r < p.a.rows) p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)sum[b] >> (p.a.shift + 4));
+                        for (int b = 0; b < OUTS; ++b)
+#pragma unroll
+                            for (int w = 0; w < WS; ++w)
+#pragma unroll
+                                for (int l = 0; l < LS; ++l) {
+                                    // (a warp too many repeats the last; a block's own memory is rank 0 of one)
+                                    const uint32_t at = from[b] + (uint32_t)((min(w0 + w, wpr - 1) * rt * AC + l * TP) * PS * 8);
+                                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][w][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
+                                }
+#pragma unroll
+                        for (int b = 0; b < OUTS; ++b)
+#pragma unroll
+                            for (int w = 0; w < WS; ++w)
+#pragma unroll
+                                for (int l = 0; l < LS; ++l) sum[b] += w0 + w < wpr ? v[b][w][l] << (PACK ? 8 * l : 0) : 0;
+                    }
+#pragma unroll
+                for (int b = 0; b < OUTS; ++b) {
+                    const int o = o0 + b * p.cs * THREADS, tok = (int)((unsigned)o / by), r = row_first + o - tok * rows_round;
+                    if (o < outs && r < p.a.rows) p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)sum[b] >> (p.a.shift + 4));
+                }
             }
-        }
+        };
+        if (outs <= p.cs * THREADS) add_up(Int<1>(), Int<4>());
+        else add_up(Int<8>(), Int<1>());
         // the sums and the activations may be overwritten (and no block leaves while another reads from it)
         __syncwarp();
         if (p.cs > 1) {
