@@ -129,7 +129,14 @@ int64_t __mind_b200_matmul_mm_i16(int64_t a, int64_t b, int64_t c, int64_t m, in
  * x: tokens x cols, y: tokens x rows int32.  The _grouped forms have one matrix per expert (w:
  * experts x rows x ceil(cols / 2), scale: experts x rows x groups), m output rows grouped by
  * `offsets`, and read row rows_of[p] of x (x_rows x cols) for output row p, or row p where rows_of
- * is 0; offsets, rows_of and untouched rows are as for matmul_grouped_i8. */
+ * is 0; offsets, rows_of and untouched rows are as for matmul_grouped_i8.
+ *
+ * Device scratch (see mind_b200_reserve) is used where an operand has to be laid out first: by
+ * matmul_grouped_i8* for m x ceil16(k) bytes of gathered or unaligned rows of A and for an unaligned
+ * B (its rows padded to 16 bytes), by gemv_w4_* for weights whose rows are no multiple of 16 bytes or
+ * whose base is not 16-byte aligned, by expert_plan for at most 320 KB above 16384 ids.  As with every
+ * call of this library, calls that use scratch on one device must not run at the same time: two graphs
+ * that hold such calls are replayed one after the other. */
 int64_t __mind_b200_expert_plan(int64_t ids, int64_t offsets, int64_t rows, int64_t place, int64_t count,
                                 int64_t experts, int64_t per);
 int64_t __mind_b200_matmul_grouped_i8(int64_t a, int64_t rows, int64_t b, int64_t offsets, int64_t scale, int64_t c,
@@ -250,6 +257,9 @@ int64_t mind_b200_shutdown(void);
  * 14 = Q16.16 GEMM only: the two-kernel hybrid in its earlier form, floor(a * (b & 0xffff) / 65536)
  * on the FP64 pipe beside seven limb products (default: floor((a & 0xffff) * (b & 0xffff) / 65536)
  * on the FP32 pipe beside eleven).
+ * For the products of quantised language models: 1 = the CUDA-core cross-check kernels of
+ * gemv_w4_* and matmul_grouped_i8*; 2 / 3 / 10 = matmul_grouped_i8* on 256-row tiles of CTA pairs /
+ * on 128-row tiles / on 32-row tiles, whatever the shape.
  * Every path gives identical bytes.  The setting is process-wide and meant for tests and
  * measurements; a call that is already running keeps the kernels it chose. */
 int64_t mind_b200_set_gemm_path(int64_t path);
