@@ -18,9 +18,11 @@ def addr(x) -> int:
     """Raw address of a numpy array, a torch tensor, or an int passed through."""
     if type(x) is int:
         return x
-    ptr = getattr(x, "data_ptr", None)  # tensors first: launch-bound callers pass several per call
-    if ptr is not None and x.is_contiguous():
-        return ptr()
+    try:  # tensors first: launch-bound callers pass several per call
+        if x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, (int, np.integer)):
         return int(x)
     if isinstance(x, np.ndarray):

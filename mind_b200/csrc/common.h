@@ -315,10 +315,16 @@ struct GroupedArgs {
 };
 int64_t launch_gemm_grouped_i8(DeviceCtx* ctx, const GroupedArgs& g);
 // dst[i] = row idx[i] (idx null: i) of src, padded with zeros to `pitch` bytes (a multiple of 16); a row
-// outside [0, src_rows) is zeros.  A kernel launched behind it with programmatic serialization starts
-// when everything before the copy is complete, and must wait for the copy itself.
-int64_t launch_copy_rows(DeviceCtx* ctx, const int8_t* src, const int32_t* idx, int8_t* dst, int64_t rows, int64_t cols,
-                         int64_t pitch, int64_t src_rows);
+// outside [0, src_rows) is zeros.  One launch for one or two of them.  A kernel launched behind it with
+// programmatic serialization starts when everything before the copies is complete, and must wait for the
+// copies themselves.
+struct CopyJob {
+    const int8_t* src;
+    const int32_t* idx;
+    int8_t* dst;
+    int64_t rows, cols, pitch, src_rows;
+};
+int64_t launch_copy_rows(DeviceCtx* ctx, const CopyJob& a, const CopyJob* b);
 // Tensor map over `experts` row-major 8-bit matrices [rows][cols] of row pitch `pitch`, one behind the
 // other: boxes of 128 columns by box_rows rows in the 128-byte swizzle.  Cached per thread.
 int64_t make_tmap_stack(CUtensorMap* tm, const void* base, int64_t cols, int64_t rows, int64_t experts, int64_t pitch,

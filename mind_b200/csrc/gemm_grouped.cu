@@ -80,23 +80,29 @@ gemm_grouped_simt_kernel(const GroupedArgs g) {
 // dst[i][0 .. pitch) = src[idx ? idx[i] : i][0 .. cols), zeros behind; a row outside [0, src_rows) is
 // zeros.  A warp takes a row, a lane 16 bytes at a time; a source that is not 16-byte aligned is read
 // as the aligned words around the bytes (only words that lie wholly inside src) and shifted together.
-// Bound by memory: cols read, pitch written.
+// Bound by memory: cols read, pitch written.  One launch may copy two matrices: the first `first_blocks`
+// blocks one, the others the other.
 __global__ void __launch_bounds__(256)
-copy_rows_kernel(const int8_t* __restrict__ src, const int32_t* __restrict__ idx, int8_t* __restrict__ dst, int64_t rows,
-                 int64_t cols, int64_t pitch, int64_t src_rows) {
+copy_rows_kernel(const CopyJob job0, const CopyJob job1, int first_blocks) {
     // Everything before this kernel is complete here, and the product behind it may start only now:
     // it relies on that for all that this kernel does not write.
     griddep_wait();
     griddep_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const int64_t warp = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
-    const int64_t nwarps = ((int64_t)gridDim.x * blockDim.x) >> 5;
+    const bool second = (int)blockIdx.x >= first_blocks;
+    const CopyJob job = second ? job1 : job0;
+    const int block = (int)blockIdx.x - (second ? first_blocks : 0), blocks = second ? (int)gridDim.x - first_blocks : first_blocks;
+    const int64_t warp = (block * (int64_t)blockDim.x + threadIdx.x) >> 5;
+    const int64_t nwarps = ((int64_t)blocks * blockDim.x) >> 5;
+    const int8_t* const src = job.src;
+    const int32_t* const idx = job.idx;
+    const int64_t rows = job.rows, cols = job.cols, pitch = job.pitch, src_rows = job.src_rows;
     const int8_t* const end = src + src_rows * cols;
     for (int64_t i = warp; i < rows; i += nwarps) {
         const int64_t r = idx ? idx[i] : i;
         const bool inside = r >= 0 && r < src_rows;
         const int8_t* const row = src + (inside ? r : 0) * cols;
-        int8_t* const to = dst + i * pitch;
+        int8_t* const to = job.dst + i * pitch;
         const int off = (int)(reinterpret_cast<uintptr_t>(row) & 15);
 #pragma unroll 4
         for (int64_t c = lane * 16; c < pitch; c += 512) {
@@ -137,12 +143,20 @@ copy_rows_kernel(const int8_t* __restrict__ src, const int32_t* __restrict__ idx
 
 }  // namespace
 
-int64_t launch_copy_rows(DeviceCtx* ctx, const int8_t* src, const int32_t* idx, int8_t* dst, int64_t rows, int64_t cols,
-                         int64_t pitch, int64_t src_rows) {
-    int64_t blocks = (rows + 7) / 8;
-    if (blocks > (int64_t)ctx->sm_count * 8) blocks = (int64_t)ctx->sm_count * 8;
+int64_t launch_copy_rows(DeviceCtx* ctx, const CopyJob& a, const CopyJob* b) {
+    const int64_t most = (int64_t)ctx->sm_count * 8;
+    auto blocks_of = [](const CopyJob& j) { return (j.rows + 7) / 8; };
+    int64_t na = blocks_of(a), nb = b ? blocks_of(*b) : 0;
+    if (na + nb > most) {  // shared out by the bytes
+        const double wa = (double)a.rows * a.pitch, wb = b ? (double)b->rows * b->pitch : 0.0;
+        if (b) {
+            nb = (int64_t)(most * (wb / (wa + wb)));
+            nb = nb < 1 ? 1 : (nb > most - 1 ? most - 1 : nb);
+        }
+        na = most - nb;
+    }
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3((unsigned)blocks, 1, 1);
+    lc.gridDim = dim3((unsigned)(na + nb), 1, 1);
     lc.blockDim = dim3(256, 1, 1);
     lc.stream = ctx->stream;
     cudaLaunchAttribute at[1];
@@ -150,7 +164,7 @@ int64_t launch_copy_rows(DeviceCtx* ctx, const int8_t* src, const int32_t* idx, 
     at[0].val.programmaticStreamSerializationAllowed = 1;
     lc.attrs = at;
     lc.numAttrs = 1;
-    MB200_CUDA(cudaLaunchKernelEx(&lc, copy_rows_kernel, src, idx, dst, rows, cols, pitch, src_rows));
+    MB200_CUDA(cudaLaunchKernelEx(&lc, copy_rows_kernel, a, b ? *b : a, (int)na));
     count_launch();
     return check_launch("copy_rows_kernel");
 }
@@ -679,20 +693,19 @@ int64_t launch_gemm_grouped_i8(DeviceCtx* ctx, const GroupedArgs& g) {
         if (!a_direct || !b_direct) {
             const size_t sa = a_direct ? 0 : (size_t)g.m * pa, sb = b_direct ? 0 : (size_t)b_rows * pb;
             MB200_TRY(arena_reserve(ctx, ctx->scratch, align_up(sa, 1024) + align_up(sb, 1024) + 2048));
+            CopyJob ja, jb;
             if (!b_direct) {
-                int8_t* to = static_cast<int8_t*>(arena_take(ctx->scratch, sb));
-                MB200_TRY(launch_copy_rows(ctx, g.b, nullptr, to, b_rows, b_cols, pb, b_rows));
-                b = to;
+                jb = CopyJob{g.b, nullptr, static_cast<int8_t*>(arena_take(ctx->scratch, sb)), b_rows, b_cols, pb, b_rows};
+                b = jb.dst;
             }
             if (!a_direct) {
-                int8_t* to = static_cast<int8_t*>(arena_take(ctx->scratch, sa));
-                MB200_TRY(launch_copy_rows(ctx, g.a, g.rows, to, g.m, g.k, pa, g.a_rows));
-                a = to;
+                ja = CopyJob{g.a, g.rows, static_cast<int8_t*>(arena_take(ctx->scratch, sa)), g.m, g.k, pa, g.a_rows};
+                a = ja.dst;
             }
+            MB200_TRY(launch_copy_rows(ctx, a_direct ? jb : ja, !a_direct && !b_direct ? &jb : nullptr));
         }
-        // The copy of A is the last launch before the product, and B (copied before it, or the caller's) is
-        // complete when that copy lets the product start.
-        const bool early = !a_direct;
+        // Where the copy makes A alone, B is complete when it lets the product start.
+        const bool early = !a_direct && b_direct;
         return g.bt ? launch_grouped_any<false>(ctx, g, a, pa, b, pb, early)
                     : launch_grouped_any<true>(ctx, g, a, pa, b, pb, early);
     }

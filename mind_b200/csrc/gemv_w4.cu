@@ -209,7 +209,7 @@ int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
         const size_t size = (size_t)(a.experts * a.rows) * pitch;
         MB200_TRY(arena_reserve(ctx, ctx->scratch, size + 2048));
         int8_t* to = static_cast<int8_t*>(arena_take(ctx->scratch, size));
-        MB200_TRY(launch_copy_rows(ctx, w, nullptr, to, a.experts * a.rows, bytes, pitch, a.experts * a.rows));
+        MB200_TRY(launch_copy_rows(ctx, CopyJob{w, nullptr, to, a.experts * a.rows, bytes, pitch, a.experts * a.rows}, nullptr));
         w = to;
     }
     CUtensorMap tm;
