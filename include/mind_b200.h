@@ -258,8 +258,8 @@ int64_t mind_b200_shutdown(void);
  * on the FP64 pipe beside seven limb products (default: floor((a & 0xffff) * (b & 0xffff) / 65536)
  * on the FP32 pipe beside eleven).
  * For the products of quantised language models: 1 = the CUDA-core cross-check kernels of
- * gemv_w4_* and matmul_grouped_i8*; 2 / 3 / 10 = matmul_grouped_i8* on 256-row tiles of CTA pairs /
- * on 128-row tiles / on 32-row tiles, whatever the shape.
+ * gemv_w4_* and matmul_grouped_i8*; 2 / 3 / 5 / 10 = matmul_grouped_i8* on 256 x 256 tiles of CTA
+ * pairs / on 128 x 256 / 128 x 128 / 32 x 128 tiles, whatever the shape.
  * Every path gives identical bytes.  The setting is process-wide and meant for tests and
  * measurements; a call that is already running keeps the kernels it chose. */
 int64_t mind_b200_set_gemm_path(int64_t path);

@@ -657,10 +657,11 @@ int64_t launch_grouped_tc(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a,
 template <bool BMN>
 int64_t launch_grouped_any(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a, int64_t pa, const int8_t* b, int64_t pb,
                            bool early) {
-    // (a kernel may be asked for by name: mind_b200_set_gemm_path 10 / 3 / 2)
+    // (a kernel may be asked for by name: mind_b200_set_gemm_path 10 / 5 / 3 / 2)
     const int pair = tuning().pair_mode.load(), small = tuning().small_tile.load();
     if (small == 1) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
     if (pair == 2) return launch_grouped_tc<128, 256, 2, BMN>(ctx, g, a, pa, b, pb, early);
+    if (pair == 1 && tuning().force_transpose.load()) return launch_grouped_tc<128, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
     if (pair == 1) return launch_grouped_tc<128, 256, 1, BMN>(ctx, g, a, pa, b, pb, early);
     // The host knows the rows and the experts, not how the rows are spread: tiles are counted as if every
     // expert had the average, half of its last tile empty.
@@ -668,9 +669,12 @@ int64_t launch_grouped_any(DeviceCtx* ctx, const GroupedArgs& g, const int8_t* a
     const double avg = m / g.experts;
     const double single_tiles = (m / 128 + half) * n256, pair_tiles = (m / 256 + half) * n256;
     // 32-row tiles where the weights are most of the traffic (2048 x 2816, 64 experts: 58.5 us against 58.2 of
-    // 128-row tiles at 8 rows an expert, 70 against 63 at 16), or where the wide tiles would leave SMs idle
-    // (4096 x 1024, 8 experts: 16.4 against 21 us at 32 rows an expert).
-    if (avg <= 8 || (avg <= 48 && single_tiles < ctx->sm_count)) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
+    // 128-row tiles at 8 rows an expert, 70 against 63 at 16; with fewer rows they are ahead).
+    if (avg <= 8) return launch_grouped_tc<32, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
+    // 128 x 128 tiles while they fit one wave: twice the CTAs, half the epilogue (4096 x 1024, 8 experts, 512
+    // rows: 16.6 us against 21.0 of 128 x 256; in more than a wave, 4096 x 2048, 1024 rows: 26.6 against 23.7).
+    if ((m / 128 + half) * (double)((g.n + 127) / 128) <= ctx->sm_count)
+        return launch_grouped_tc<128, 128, 1, BMN>(ctx, g, a, pa, b, pb, early);
     // Pairs of CTAs move a third less per product (32768 x 4096 x 4096: 390 us against 443), unless their
     // coarser tiles cost a wave (4096 x 4096 x 2048, 8 experts: 42 us in three waves against 38 in two).
     const double single_waves = single_tiles / ctx->sm_count, pair_waves = pair_tiles / (ctx->sm_count / 2);

@@ -235,7 +235,7 @@ def test_native_sources_file_forwards(tmp_path, library, status):
 
 # ------------------------------------------------------------------------------- on a GPU
 PATHS = {"default": 0, "cross-check": 1}
-GROUPED_PATHS = {**PATHS, "pairs": 2, "single": 3, "small": 10}
+GROUPED_PATHS = {**PATHS, "pairs": 2, "single": 3, "square": 5, "small": 10}
 
 
 @pytest.fixture(params=list(PATHS))
@@ -248,7 +248,7 @@ def path(request, gpu):
 
 @pytest.fixture(params=list(GROUPED_PATHS))
 def grouped_path(request, gpu):
-    """The grouped product's kernels: by shape, cross-check, 256-row tiles on CTA pairs, 128-row, 32-row tiles."""
+    """The grouped product's kernels: by shape, cross-check, 256 x 256 tiles on CTA pairs, 128 x 256, 128 x 128, 32 x 128."""
     gpu.set_gemm_path(GROUPED_PATHS[request.param])
     yield request.param
     gpu.set_gemm_path(0)
