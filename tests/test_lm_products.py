@@ -600,3 +600,129 @@ def test_operands_of_another_device_are_refused(torch_gpu, gpu):
     y = torch.zeros(16, dtype=torch.int32, device="cuda:1")
     z = torch.zeros(64, dtype=torch.int8, device="cuda:0")
     refused(mind_b200.ERR_INVALID, gpu.gemv_w4_i8, z, z, z, y, 1, 1, 32, 32, 0)
+
+
+@pytest.mark.gpu
+def test_weights_past_32_bits(torch_gpu, gpu):
+    """Stacks of weights of more than 2^31 bytes, and an output of more than 2^31 elements."""
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def some(shape, dtype=torch.int8):
+        return torch.randint(-128, 128, shape, generator=gen, device="cuda", dtype=torch.int16).to(dtype)
+
+    # 4-bit: 70 experts of 4096 x 16384
+    experts, rows, cols, group = 70, 4096, 16384, 128
+    w, s, x = some((experts, rows, cols // 2)), some((experts, rows, cols // group), torch.int16), some((3, cols))
+    assert w.numel() > 2 ** 31
+    offsets = torch.zeros(experts + 1, **i32)
+    offsets[1:] = 1
+    offsets[-1] = 3
+    y = torch.zeros((3, rows), **i32)
+    gpu.gemv_w4_grouped_i8(w, s, x, None, offsets, y, 3, rows, cols, group, 8, experts, 3)
+    got = y.cpu().numpy()
+    for p, e in ((0, 0), (1, experts - 1), (2, experts - 1)):
+        want = ref_w4(w[e].cpu().numpy(), s[e].cpu().numpy(), x[p:p + 1].cpu().numpy(), cols, group, 8)
+        assert np.array_equal(got[p:p + 1], want), p
+    del w
+
+    # int8: nine experts of 16384 x 16384, both orientations
+    experts, k, n = 9, 16384, 16384
+    b, a = some((experts, k, n)), some((40, k))
+    assert b.numel() > 2 ** 31
+    offsets = torch.full((experts + 1,), 7, **i32)
+    offsets[0] = 0
+    offsets[-1] = 40
+    c = torch.zeros((40, n), **i32)
+    for bt, fn in ((False, gpu.matmul_grouped_i8), (True, gpu.matmul_grouped_i8_bt)):
+        fn(a, None, b, offsets, None, c, 40, k, n, experts, 40)
+        for lo, hi, e in ((0, 7, 0), (7, 40, experts - 1)):
+            part = b[e, -96:].t() if bt else b[e, :, -96:]
+            want = torch.matmul(a[lo:hi].double(), part.double()).long().to(torch.int32)
+            assert torch.equal(c[lo:hi, -96:], want), (bt, e)
+    del b, c
+
+    # an output of 2.2e9 elements
+    m, k, n = 68000, 32, 32256
+    a, b = some((m, k)), some((2, k, n))
+    offsets = torch.tensor([0, 30001, m], **i32)
+    c = torch.zeros((m, n), **i32)
+    assert c.numel() > 2 ** 31
+    gpu.matmul_grouped_i8(a, None, b, offsets, None, c, m, k, n, 2, m)
+    for lo, hi, e in ((0, 5, 0), (29990, 30001, 0), (30001, 30010, 1), (m - 9, m, 1)):
+        want = torch.matmul(a[lo:hi].double(), b[e].double()).long().to(torch.int32)
+        assert torch.equal(c[lo:hi], want), (lo, e)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count,experts", [(16384, 17), (16385, 17), (3_000_000, 384), (2_000_000, 2500)])
+def test_expert_plan_large(torch_gpu, gpu, count, experts):
+    """Both forms at their border, and long batches, against a stable sort."""
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(count)
+    ids = torch.randint(-1, experts, (count,), generator=gen, device="cuda", dtype=torch.int32)
+    offsets, rows, place = (torch.full((n,), CANARY, dtype=torch.int32, device="cuda") for n in (experts + 1, count, count))
+    gpu.expert_plan(ids, offsets, rows, place, count, experts, 3)
+    key = torch.where(ids >= 0, ids, experts).long()
+    order = torch.sort(key, stable=True).indices
+    kept = int((ids >= 0).sum())
+    assert torch.equal(offsets.long(), torch.cat([torch.zeros(1, dtype=torch.long, device="cuda"),
+                                                  torch.bincount(key, minlength=experts + 1)[:experts].cumsum(0)]))
+    assert torch.equal(rows[:kept].long(), order[:kept] // 3) and bool((rows[kept:] == CANARY).all())
+    want = torch.full((count,), -1, dtype=torch.int32, device="cuda")
+    want[order[:kept]] = torch.arange(kept, dtype=torch.int32, device="cuda")
+    assert torch.equal(place, want)
+
+
+@pytest.mark.gpu
+def test_two_graphs_one_after_the_other(torch_gpu, gpu):
+    """Two captured layers that share the library's scratch (gathered rows, odd columns), replayed in turn and
+    mixed with eager calls of a third."""
+    torch = torch_gpu
+    layers = [expert_layer(gpu, torch, np.random.default_rng(s), 50, 2, 5, 130 + s, 95) for s in (1, 2, 3)]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    with torch.cuda.stream(stream):
+        gpu.set_stream(stream.cuda_stream)
+        for _, run, _ in layers:
+            run()
+        stream.synchronize()
+        for _, run, _ in layers[:2]:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                run()
+            graphs.append(graph)
+        for d, _, _ in layers:
+            for name in ("offsets", "rows", "place", "h", "y"):
+                d[name].fill_(CANARY)
+        for _ in range(3):
+            graphs[0].replay()
+            layers[2][1]()
+            graphs[1].replay()
+        stream.synchronize()
+    for layer in layers:
+        layer[2]()
+    gpu.set_stream(0)
+
+
+@pytest.mark.gpu
+def test_other_streams(torch_gpu, gpu):
+    """Each call's operands are made on the stream it runs on, without a wait in between."""
+    torch = torch_gpu
+    layers = []
+    for s in (1, 2):
+        stream = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            gpu.set_stream(stream.cuda_stream)
+            layer = expert_layer(gpu, torch, np.random.default_rng(s), 60, 2, 6, 256, 320)
+            for name in ("x", "w", "s"):  # queued on the same stream right before the calls
+                layer[0][name].add_(1).sub_(1)
+            layer[1]()
+            layers.append(layer)
+    for layer in layers:
+        layer[2]()
