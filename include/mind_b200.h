@@ -116,8 +116,8 @@ int64_t __mind_b200_matmul_mm_i16(int64_t a, int64_t b, int64_t c, int64_t m, in
  * a: a_rows x k int8 (a_rows == m where rows is 0); b: experts x k x n int8, for the _bt form
  * experts x n x k; c: m x n int32.  rows of A outside [0, a_rows) count as zeros.  Rows of C that
  * belong to no expert are left as they were.  offsets is int32[experts + 1], a running sum within
- * [0, m]; a host array that is not one is refused, in device memory each bound is taken no lower
- * than the one before and no higher than m.
+ * [0, m]; a pageable host array that is not one is refused, in device or pinned memory each bound is
+ * taken no lower than the one before and no higher than m.
  *
  * gemv_w4_* multiply 4-bit weights by a few tokens' activations (int8, int16 or Q16.16):
  *   y[t,r] = (i32)( ( sum_g (i64)scale[r,g] * sum_{k in g} W[r,k] * x[t,k] ) >> shift )

@@ -799,13 +799,14 @@ int64_t check_extent(int64_t a, int64_t b, int64_t c) {
     return 0;
 }
 
-// Offsets in host memory can be looked at: they must be a running sum within [0, m].  (Those in
-// device memory are bounded by the kernels.)
+// Offsets in pageable host memory can be looked at: they must be a running sum within [0, m].  (Those in
+// device or pinned memory may be the work of something that the stream has yet to do: they are bounded by
+// the kernels.)
 int64_t check_host_offsets(const int32_t* offsets, int64_t experts, int64_t m) {
     cudaPointerAttributes at;
     if (cudaPointerGetAttributes(&at, offsets) != cudaSuccess)
         cudaGetLastError();  // memory CUDA does not know, or no device at all: an ordinary host address
-    else if (at.type == cudaMemoryTypeDevice || at.type == cudaMemoryTypeManaged)
+    else if (at.type != cudaMemoryTypeUnregistered)
         return 0;
     int64_t before = 0;
     for (int64_t e = 0; e <= experts; ++e) {

@@ -726,3 +726,26 @@ def test_other_streams(torch_gpu, gpu):
             layers.append(layer)
     for layer in layers:
         layer[2]()
+
+
+@pytest.mark.gpu
+def test_pinned_offsets_written_in_stream_order(torch_gpu, gpu):
+    """Offsets in pinned memory may still be on their way when the call is made: they are not looked at then."""
+    torch = torch_gpu
+    rng = np.random.default_rng(9)
+    m, k, n, experts = 20, 64, 48, 3
+    a, b = rng.integers(-128, 128, (m, k), dtype=np.int8), rng.integers(-128, 128, (experts, k, n), dtype=np.int8)
+    offsets = np.array([0, 6, 6, m], dtype=np.int32)
+    da, db, do = dev(torch, a, b, offsets)
+    pinned = torch.full((experts + 1,), CANARY, dtype=torch.int32).pin_memory()
+    c = torch.full((m, n), CANARY, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    gpu.set_stream(stream.cuda_stream)
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        pinned.copy_(do, non_blocking=True)
+        gpu.matmul_grouped_i8(da, None, db, pinned, None, c, m, k, n, experts, m)
+    gpu.set_stream(0)
+    want = ref_grouped(a, None, b, offsets, None, np.full((m, n), CANARY, np.int32), 0, False)
+    assert np.array_equal(c.cpu().numpy(), want)
