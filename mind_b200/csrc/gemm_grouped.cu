@@ -272,9 +272,13 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
     {
         const int per = (p.experts + GT_THREADS - 1) / GT_THREADS;
         const int e0 = min((int)threadIdx.x * per, p.experts), e1 = min(e0 + per, p.experts);
-        int mx = min(max(p.offsets[0], 0), p.m);
+        int mx = min(max(__ldcg(p.offsets), 0), p.m);  // (from L2: this kernel may start before the copy's end)
         const int first = mx;
-        for (int e = e0; e < e1; ++e) mx = max(mx, min(p.offsets[e + 1], p.m));
+        for (int e = e0; e < e1; ++e) {
+            const int at = min(__ldcg(p.offsets + e + 1), p.m);
+            bound[e + 1] = at;
+            mx = max(mx, at);
+        }
         int incl = mx;
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -287,7 +291,7 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
         for (int w = 0; w < warp; ++w) before = max(before, warp_max[w]);
         int tiles = 0, lo = before;
         for (int e = e0; e < e1; ++e) {
-            const int hi = max(lo, min(p.offsets[e + 1], p.m));
+            const int hi = max(lo, bound[e + 1]);
             bound[e + 1] = hi;
             tiles += tiles_of(hi - lo, TILE_M);
             lo = hi;

@@ -229,7 +229,10 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         const int e0 = min((int)threadIdx.x * per, experts), e1 = min(e0 + per, experts);
         const int first = offset(0);
         int mx = first;
-        for (int e = e0; e < e1; ++e) mx = max(mx, offset(e + 1));
+        for (int e = e0; e < e1; ++e) {
+            bound[e + 1] = offset(e + 1);
+            mx = max(mx, bound[e + 1]);
+        }
         int incl = mx;
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, incl, o);
@@ -242,7 +245,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         for (int w = 0; w < warp; ++w) before = max(before, misc[4 + w]);
         int blocks = 0, lo = before;
         for (int e = e0; e < e1; ++e) {
-            const int hi = max(lo, offset(e + 1));
+            const int hi = max(lo, bound[e + 1]);
             bound[e + 1] = hi;
             blocks += (hi - lo + p.tb - 1) / p.tb;
             lo = hi;
