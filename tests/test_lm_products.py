@@ -749,3 +749,19 @@ def test_pinned_offsets_written_in_stream_order(torch_gpu, gpu):
     gpu.set_stream(0)
     want = ref_grouped(a, None, b, offsets, None, np.full((m, n), CANARY, np.int32), 0, False)
     assert np.array_equal(c.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("experts", [1, 2, 63, 64, 255, 1025, 4096])
+@pytest.mark.parametrize("count", [31, 128, 129, 256, 257, 512, 513, 1025, 2047, 2049, 8192, 8193, 16384, 16385, 40007])
+def test_expert_plan_borders(gpu, count, experts):
+    """Where the kernel takes another block, more warps or a second launch; few and many ids of one expert."""
+    rng = np.random.default_rng(count + 100003 * experts)
+    any_id = rng.integers(-1, experts + 1, count, dtype=I32)
+    runs = np.sort(rng.integers(0, experts, count, dtype=I32))[::-1].copy()
+    for ids in (any_id, runs, np.full(count, experts - 1, I32), np.full(count, experts, I32)):
+        offsets, rows, place = (np.full(n, CANARY, I32) for n in (experts + 1, count, count))
+        want = ref_plan(ids, experts, 2, rows)
+        gpu.expert_plan(ids, offsets, rows, place, count, experts, 2)
+        for got, expected in zip((offsets, rows, place), want):
+            assert np.array_equal(got, expected)
