@@ -51,7 +51,9 @@ expert_plan_kernel(const int32_t* ids, int32_t* __restrict__ offsets, int32_t* _
     const bool cluster = phase == 0 && blocks > 1;  // the grid is one cluster
     int32_t* const total = hist + warps * experts;
     int32_t* const prior = total + experts;
-    if (phase != 1) griddep_launch_dependents();
+    // (The second launch says nothing: blocks of the kernel behind it, waiting beside it, moved its own blocks
+    // off their SMs - 300126 ids over 160 experts 11.2 us against 9.1; other sizes differ by 0.4 at most.)
+    if (phase == 0) griddep_launch_dependents();
     for (int i = threadIdx.x; i < (warps + 2) * experts; i += blockDim.x) hist[i] = 0;
     if (threadIdx.x == 0) carry = 0;
     // The ids may be the work of the kernel before this one.  The first of two launches lets the second
