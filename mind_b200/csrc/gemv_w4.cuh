@@ -575,6 +575,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         const int row_first = (u - q * p.row_rounds) * rows_round;
         const int outs = rows_round * ntok;
         const unsigned by = (unsigned)rows_round;
+        const int all = p.cs * wpr;
         // A thread adds up OUTS outputs at a time, the partial sums of WS warps in each, so that enough (remote)
         // loads travel together: few outputs and many warps, or the other way round.
         auto add_up = [&](auto outs_at_a_time, auto warps_at_a_time) {
@@ -588,26 +589,32 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
                     sum[b] = 0;
                     from[b] = smem_u32(part + ((rr >> 4) * AC + tok) * PS + (rr & 15));
                 }
-                for (int c = 0; c < p.cs; ++c)
-                    for (int w0 = 0; w0 < wpr; w0 += WS) {
-                        uint64_t v[OUTS][WS][LS];
+                // the warps of all the cluster's blocks as one list, WS of them at a time
+                int c = 0, w = 0;
+                for (int j0 = 0; j0 < all; j0 += WS) {
+                    uint64_t v[OUTS][WS][LS];
+#pragma unroll
+                    for (int k = 0; k < WS; ++k) {
 #pragma unroll
                         for (int b = 0; b < OUTS; ++b)
 #pragma unroll
-                            for (int w = 0; w < WS; ++w)
-#pragma unroll
-                                for (int l = 0; l < LS; ++l) {
-                                    // (a warp too many repeats the last; a block's own memory is rank 0 of one)
-                                    const uint32_t at = from[b] + (uint32_t)((min(w0 + w, wpr - 1) * rt * AC + l * TP) * PS * 8);
-                                    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][w][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
-                                }
-#pragma unroll
-                        for (int b = 0; b < OUTS; ++b)
-#pragma unroll
-                            for (int w = 0; w < WS; ++w)
-#pragma unroll
-                                for (int l = 0; l < LS; ++l) sum[b] += w0 + w < wpr ? v[b][w][l] << (PACK ? 8 * l : 0) : 0;
+                            for (int l = 0; l < LS; ++l) {
+                                // (one too many repeats the last; a block's own memory is rank 0 of one)
+                                const uint32_t at = from[b] + (uint32_t)((w * rt * AC + l * TP) * PS * 8);
+                                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][k][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
+                            }
+                        if (j0 + k + 1 < all) {
+                            c += w + 1 == wpr ? 1 : 0;
+                            w = w + 1 == wpr ? 0 : w + 1;
+                        }
                     }
+#pragma unroll
+                    for (int k = 0; k < WS; ++k)
+#pragma unroll
+                        for (int b = 0; b < OUTS; ++b)
+#pragma unroll
+                            for (int l = 0; l < LS; ++l) sum[b] += j0 + k < all ? v[b][k][l] << (PACK ? 8 * l : 0) : 0;
+                }
 #pragma unroll
                 for (int b = 0; b < OUTS; ++b) {
                     const int o = o0 + b * p.cs * THREADS, tok = (int)((unsigned)o / by), r = row_first + o - tok * rows_round;
@@ -615,7 +622,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
                 }
             }
         };
-        if (outs <= p.cs * THREADS) add_up(Int<1>(), Int<4>());
+        if (outs <= p.cs * THREADS) add_up(Int<1>(), Int<8>());
         else add_up(Int<8>(), Int<1>());
         // the sums and the activations may be overwritten (and no block leaves while another reads from it)
         __syncwarp();
