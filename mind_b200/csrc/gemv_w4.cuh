@@ -90,10 +90,6 @@ __device__ __forceinline__ void mma_step(int (&d)[4], const uint32_t (&a)[4], ui
     else if (keep) mma<SIGNED, false, true>(d, a, b0, b1);
     else mma<SIGNED, false, false>(d, a, b0, b1);
 }
-template <int N>
-struct Int {
-    static constexpr int value = N;
-};
 // 4 * N bytes of shared memory.
 template <int N>
 __device__ __forceinline__ void lds(uint32_t (&v)[N], uint32_t addr) {
@@ -576,54 +572,37 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         const int outs = rows_round * ntok;
         const unsigned by = (unsigned)rows_round;
         const int all = p.cs * wpr;
-        // A thread adds up OUTS outputs at a time, the partial sums of WS warps in each, so that enough (remote)
-        // loads travel together: few outputs and many warps, or the other way round.
-        auto add_up = [&](auto outs_at_a_time, auto warps_at_a_time) {
-            constexpr int OUTS = decltype(outs_at_a_time)::value, WS = decltype(warps_at_a_time)::value, LS = PACK ? L : 1;
-            for (int o0 = (int)rank * THREADS + threadIdx.x; o0 < outs; o0 += OUTS * p.cs * THREADS) {
-                uint64_t sum[OUTS];
-                uint32_t from[OUTS];
+        // A thread adds up an output: the partial sums of all the cluster's warps as one list, four (remote) loads
+        // at a time.  (Eight: 24.4 against 23.0 us for 8192 x 8192 Q16.16 of eight tokens; eight outputs of one
+        // warp each 25.9.  Several of these forms, chosen by the sizes, are behind one again: their code is long.)
+        constexpr int AT_ONCE = 4, LS = PACK ? L : 1;
+        for (int o = (int)rank * THREADS + threadIdx.x; o < outs; o += p.cs * THREADS) {
+            const int tok = (int)((unsigned)o / by), rr = o - tok * rows_round, r = row_first + rr;
+            const uint32_t from = smem_u32(part + ((rr >> 4) * AC + tok) * PS + (rr & 15));
+            uint64_t sum = 0;
+            int c = 0, w = 0;
+            for (int j0 = 0; j0 < all; j0 += AT_ONCE) {
+                uint64_t v[AT_ONCE][LS];
 #pragma unroll
-                for (int b = 0; b < OUTS; ++b) {
-                    const int o = min(o0 + b * p.cs * THREADS, outs - 1), tok = (int)((unsigned)o / by), rr = o - tok * rows_round;
-                    sum[b] = 0;
-                    from[b] = smem_u32(part + ((rr >> 4) * AC + tok) * PS + (rr & 15));
-                }
-                // the warps of all the cluster's blocks as one list, WS of them at a time
-                int c = 0, w = 0;
-                for (int j0 = 0; j0 < all; j0 += WS) {
-                    uint64_t v[OUTS][WS][LS];
+                for (int k = 0; k < AT_ONCE; ++k) {
 #pragma unroll
-                    for (int k = 0; k < WS; ++k) {
-#pragma unroll
-                        for (int b = 0; b < OUTS; ++b)
-#pragma unroll
-                            for (int l = 0; l < LS; ++l) {
-                                // (one too many repeats the last; a block's own memory is rank 0 of one)
-                                const uint32_t at = from[b] + (uint32_t)((w * rt * AC + l * TP) * PS * 8);
-                                asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v[b][k][l]) : "r"(mapa(at, (uint32_t)c)) : "memory");
-                            }
-                        if (j0 + k + 1 < all) {
-                            c += w + 1 == wpr ? 1 : 0;
-                            w = w + 1 == wpr ? 0 : w + 1;
-                        }
+                    for (int l = 0; l < LS; ++l)  // (one too many repeats the last; a block's own memory is rank 0 of one)
+                        asm volatile("ld.shared::cluster.u64 %0, [%1];"
+                                     : "=l"(v[k][l])
+                                     : "r"(mapa(from + (uint32_t)((w * rt * AC + l * TP) * PS * 8), (uint32_t)c))
+                                     : "memory");
+                    if (j0 + k + 1 < all) {
+                        c += w + 1 == wpr ? 1 : 0;
+                        w = w + 1 == wpr ? 0 : w + 1;
                     }
-#pragma unroll
-                    for (int k = 0; k < WS; ++k)
-#pragma unroll
-                        for (int b = 0; b < OUTS; ++b)
-#pragma unroll
-                            for (int l = 0; l < LS; ++l) sum[b] += j0 + k < all ? v[b][k][l] << (PACK ? 8 * l : 0) : 0;
                 }
 #pragma unroll
-                for (int b = 0; b < OUTS; ++b) {
-                    const int o = o0 + b * p.cs * THREADS, tok = (int)((unsigned)o / by), r = row_first + o - tok * rows_round;
-                    if (o < outs && r < p.a.rows) p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)sum[b] >> (p.a.shift + 4));
-                }
+                for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+                    for (int l = 0; l < LS; ++l) sum += j0 + k < all ? v[k][l] << (PACK ? 8 * l : 0) : 0;
             }
-        };
-        if (outs <= p.cs * THREADS) add_up(Int<1>(), Int<8>());
-        else add_up(Int<8>(), Int<1>());
+            if (r < p.a.rows) p.a.y[(int64_t)(p0 + tok) * p.a.rows + r] = (int32_t)((int64_t)sum >> (p.a.shift + 4));
+        }
         // the sums and the activations may be overwritten (and no block leaves while another reads from it)
         __syncwarp();
         if (p.cs > 1) {
