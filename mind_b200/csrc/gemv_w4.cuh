@@ -379,12 +379,13 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
             p0 = bound[e_now] + (int)(i * per + min(i, extra));
             ntok = (int)per + (i < extra ? 1 : 0);
             // A thread owns groups of eight columns and takes them token by token (the block several tokens at once
-            // where the columns are few): 32 registers of loads before the first store, and
-            // all of them before the weights are asked for, behind which they would have to queue.
+            // where the columns are few): 16 or 32 registers of loads before the first store (more lengthen the
+            // code: 4096 x 4096 int8 of eight tokens 8.7 us with 16, 9.6 with 32), and the weights are asked for
+            // behind the last of them, not before, where the activations would have to queue.
             const int octs = (kb_hi - kb_lo) * (KB / 8);
             const int width = octs < THREADS ? octs : THREADS, tstep = THREADS / width;
             const int tok0 = (int)threadIdx.x / width, o0 = (int)threadIdx.x - tok0 * width;
-            constexpr int BATCH = TC <= 2 ? 2 * TC : 16 / L;
+            constexpr int BATCH = TC <= 2 ? 2 * TC : (L == 1 ? 8 : 4);
             int lo = o0, lt = tok0, so = o0, st = tok0;  // next to load, next to store: columns, token
             if (tok0 >= tstep || tok0 >= ntok) lo = so = octs;
             while (so < octs) {
