@@ -24,10 +24,10 @@
 //   across the cluster by remote reads: integer sums, so no order changes a bit, and nothing is kept in
 //   global memory.
 //
-// What bounds it.  One or two tokens: memory behind a set-up of about 5 us (28672 x 8192 int8: 25.9 us a
-// call, 4.7 TB/s of weights and scales, 0.72 of the copy bandwidth; 4096 x 4096: 6.2 us, of which the host
+// What bounds it.  One or two tokens: memory behind a set-up of about 5 us (28672 x 8192 int8: 24.7 to 25.8
+// us a call, 4.8 TB/s of weights and scales, 0.73 of the copy bandwidth; 4096 x 4096: 6.2 us, of which the host
 // needs about as much to make the call).  More: the latency of the main loop on four warps a scheduler (8192 x
-// 8192 Q16.16, eight tokens, groups of 32: 25.8 us against 5.9 us of memory time; no pipe is more than half
+// 8192 Q16.16, eight tokens, groups of 32: 22.8 us against 5.9 us of memory time; no pipe is more than half
 // busy).  MMAs run at 8.2 clocks a scheduler whatever their operands.
 #pragma once
 #include "common.h"
