@@ -61,34 +61,27 @@ struct Params {
     int* err;
 };
 
-// D (+)= A . B, 16 x 32 weights (s8) by 32 x 8 activation bytes.  FIRST: D = A . B.  KEEP: stays before
-// every later volatile statement (the refill of the slot that its operands came from).
-template <bool SIGNED, bool FIRST, bool KEEP>
+// D (+)= A . B, 16 x 32 weights (s8) by 32 x 8 activation bytes.  FIRST: D = A . B.
+template <bool SIGNED, bool FIRST>
 __device__ __forceinline__ void mma(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-#define MB200_W4_MMA(V, T, C, ...)                                                                                          \
-    asm V("mma.sync.aligned.m16n8k32.row.col.s32.s8." T ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " C ";" __VA_ARGS__)
+#define MB200_W4_MMA(T, C, ...)                                                                                          \
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8." T ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, " C ";" __VA_ARGS__)
 #define MB200_W4_IN "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1)
 #define MB200_W4_NEW : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]) : MB200_W4_IN, "r"(0)
 #define MB200_W4_ADD : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : MB200_W4_IN
-    if constexpr (SIGNED && FIRST && KEEP) MB200_W4_MMA(volatile, "s8", "{%10,%10,%10,%10}", MB200_W4_NEW);
-    else if constexpr (SIGNED && FIRST) MB200_W4_MMA(, "s8", "{%10,%10,%10,%10}", MB200_W4_NEW);
-    else if constexpr (SIGNED && KEEP) MB200_W4_MMA(volatile, "s8", "{%0,%1,%2,%3}", MB200_W4_ADD);
-    else if constexpr (SIGNED) MB200_W4_MMA(, "s8", "{%0,%1,%2,%3}", MB200_W4_ADD);
-    else if constexpr (FIRST && KEEP) MB200_W4_MMA(volatile, "u8", "{%10,%10,%10,%10}", MB200_W4_NEW);
-    else if constexpr (FIRST) MB200_W4_MMA(, "u8", "{%10,%10,%10,%10}", MB200_W4_NEW);
-    else if constexpr (KEEP) MB200_W4_MMA(volatile, "u8", "{%0,%1,%2,%3}", MB200_W4_ADD);
-    else MB200_W4_MMA(, "u8", "{%0,%1,%2,%3}", MB200_W4_ADD);
+    if constexpr (SIGNED && FIRST) MB200_W4_MMA("s8", "{%10,%10,%10,%10}", MB200_W4_NEW);
+    else if constexpr (SIGNED) MB200_W4_MMA("s8", "{%0,%1,%2,%3}", MB200_W4_ADD);
+    else if constexpr (FIRST) MB200_W4_MMA("u8", "{%10,%10,%10,%10}", MB200_W4_NEW);
+    else MB200_W4_MMA("u8", "{%0,%1,%2,%3}", MB200_W4_ADD);
 #undef MB200_W4_MMA
 #undef MB200_W4_IN
 #undef MB200_W4_NEW
 #undef MB200_W4_ADD
 }
 template <bool SIGNED>
-__device__ __forceinline__ void mma_step(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first, bool keep) {
-    if (first && keep) mma<SIGNED, true, true>(d, a, b0, b1);
-    else if (first) mma<SIGNED, true, false>(d, a, b0, b1);
-    else if (keep) mma<SIGNED, false, true>(d, a, b0, b1);
-    else mma<SIGNED, false, false>(d, a, b0, b1);
+__device__ __forceinline__ void mma_step(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, bool first) {
+    if (first) mma<SIGNED, true>(d, a, b0, b1);
+    else mma<SIGNED, false>(d, a, b0, b1);
 }
 // 4 * N bytes of shared memory.
 template <int N>
@@ -297,9 +290,9 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
         while (q >= cumb[is_e + 1]) ++is_e;
         is_row0 = ((is_u - q * p.row_rounds) * rt + my_tile) * 16;
     };
-    auto issue = [&]() {
+    auto issue = [&](bool done) {  // done: the slot's last box has been multiplied (or it never held one)
         if (is_u >= u1) return;
-        if (lead) {
+        if (lead && done) {
             mbar_arrive_expect_tx(bars + 8 * fill, BOX_BYTES);
             tma_load_3d(slots0 + fill * RING_BYTES, &tm_w, bars + 8 * fill, is_x, is_row0, is_e, policy);
         }
@@ -429,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
                 }
                 if (!asked && lo >= octs) {
                     asked = true;
-                    for (int s = 0; s < p.slots; ++s) issue();
+                    for (int s = 0; s < p.slots; ++s) issue(true);
                 }
 #pragma unroll
                 for (int b = 0; b < BATCH; ++b) {
@@ -451,7 +444,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
             }
             if (!asked) {
                 asked = true;
-                for (int s = 0; s < p.slots; ++s) issue();
+                for (int s = 0; s < p.slots; ++s) issue(true);
             }
             if (u == u0) prefetch_scales(u0, e_now);
             __syncthreads();
@@ -492,6 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
             // this lane's words of scaling f of the box lie at wbase ^ (f * 16 GB), the box's swizzle included
             const uint32_t wbase = slots0 + take * RING_BYTES + row * 128 +
                                    (((t * GB / 4) ^ row) << 4) + (t * GB % 4) * 4;
+            int used = 0;  // depends on every word of the box
 #pragma unroll
             for (int f = 0; f < FB; ++f) {
                 const int m0 = __shfl_sync(0xffffffffu, sc[0][f % NS], (lane & 28) | (h * (FB / NS) + f / NS));
@@ -523,18 +517,18 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
 #pragma unroll
                         for (int l = 0; l < LT; ++l) {
                             const uint32_t x0 = x[l][b / XP::MMAS][2 * (b % XP::MMAS)], x1 = x[l][b / XP::MMAS][2 * (b % XP::MMAS) + 1];
-                            const bool keep = f == FB - 1 && b == GB - 1 && l == LT - 1;
                             if (PACK) {  // the unsigned columns, then the signed ones
-                                mma_step<false>(acc[0], a[b], col_top ? 0u : x0, col_top ? 0u : x1, b == 0, false);
-                                mma_step<true>(acc[0], a[b], col_top ? x0 : 0u, col_top ? x1 : 0u, false, keep);
+                                mma_step<false>(acc[0], a[b], col_top ? 0u : x0, col_top ? 0u : x1, b == 0);
+                                mma_step<true>(acc[0], a[b], col_top ? x0 : 0u, col_top ? x1 : 0u, false);
                             } else if (l < L - 1) {
-                                mma_step<false>(acc[l], a[b], x0, x1, b == 0, keep);
+                                mma_step<false>(acc[l], a[b], x0, x1, b == 0);
                             } else {
-                                mma_step<true>(acc[l], a[b], x0, x1, b == 0, keep);
+                                mma_step<true>(acc[l], a[b], x0, x1, b == 0);
                             }
                         }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
+                        if (n == 0 && i == 0) used ^= acc[LT - 1][0];
                         const int m = i < 2 ? m0 : m1;
                         if (PACK || L == 1) {
                             acc64[n][i] += (int64_t)m * acc[0][i];
@@ -548,11 +542,15 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
                 }
                 xat += CSTRIDE;
             }
-            // The box's words have been multiplied (the MMAs above took them: every lane's loads are done), so
-            // its slot may be filled again.
+            // The slot may be filled again once every lane's words of the box have been USED: nothing else keeps a
+            // load of them from following the refill (the compiler sees no address in common, and an order left to
+            // it failed in the fused Q16.16 kernel).  So the refill is predicated on a vote over sums that each
+            // scaling's words went through.  They stay below 2^23 in magnitude, so bits 30 and 31 agree in all of
+            // them: the vote always succeeds, which the compiler cannot know.
+            const bool done = __all_sync(0xffffffffu, used != 0x40000000);
             take = take + 1 == p.slots ? 0 : take + 1;
             phase ^= take == 0 ? 1u : 0u;
-            issue();
+            issue(done);
             }
         }
         // ---- the round's partial sums: of wpr warps here, and of the cluster's other columns

@@ -765,3 +765,39 @@ def test_expert_plan_borders(gpu, count, experts):
         gpu.expert_plan(ids, offsets, rows, place, count, experts, 2)
         for got, expected in zip((offsets, rows, place), want):
             assert np.array_equal(got, expected)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,tokens,rows,cols,group,sets", [
+    ("i8", 1, 28672, 8192, 128, 2), ("q16", 8, 16384, 8192, 32, 3), ("q16", 8, 16384, 8192, 128, 3),
+    ("i16", 5, 12289, 5120, 64, 5), ("i8", 32, 8192, 8192, 256, 5)])
+def test_gemv_w4_slots_are_refilled_behind_their_readers(torch_gpu, gpu, kind, tokens, rows, cols, group, sets):
+    """Weights that come from memory every time (matrices larger than L2 together, taken in turn): the warps wait
+    for the boxes of their ring and refill each slot as soon as it has been multiplied."""
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(rows + group)
+
+    def some(shape, lo, hi, dtype):
+        return torch.randint(lo, hi, shape, generator=gen, device="cuda", dtype=torch.int64).to(dtype)
+
+    lim = {"i8": 2 ** 7, "i16": 2 ** 15, "q16": 2 ** 31}[kind]
+    x = some((tokens, cols), -lim, lim, {"i8": torch.int8, "i16": torch.int16, "q16": torch.int32}[kind])
+    w = [torch.randint(-128, 128, (rows, cols // 2), generator=gen, device="cuda", dtype=torch.int16).to(torch.int8)
+         for _ in range(sets)]
+    s = [some((rows, cols // group), -2 ** 15, 2 ** 15, torch.int16) for _ in range(sets)]
+    assert sets * w[0].numel() > 150_000_000  # 126 MB of L2
+    fn = getattr(gpu, f"gemv_w4_{kind}")
+    want = [torch.empty((tokens, rows), dtype=torch.int32, device="cuda") for _ in range(sets)]
+    gpu.set_gemm_path(1)
+    for i in range(sets):
+        fn(w[i], s[i], x, want[i], tokens, rows, cols, group, 9)
+    gpu.set_gemm_path(0)
+    y = torch.empty((tokens, rows), dtype=torch.int32, device="cuda")
+    wrong = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for n in range(40 * sets):
+        y.fill_(CANARY)
+        fn(w[n % sets], s[n % sets], x, y, tokens, rows, cols, group, 9)
+        wrong += (y != want[n % sets]).sum()
+    gpu.synchronize()
+    assert int(wrong) == 0
