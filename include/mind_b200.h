@@ -268,6 +268,17 @@ int64_t mind_b200_set_gemm_path(int64_t path);
  * same; 2 = every group walks N forwards; 3 = the default order with the epilogue storing rows
  * itself instead of handing its blocks to TMA stores).  Every setting gives identical bytes. */
 int64_t mind_b200_set_tile_order(int64_t group_m, int64_t raster);
+/* Shape of the gemv_w4_* kernel, for tests and measurements: blocks per cluster (1, 2, 4 or 8, which share
+ * the columns), row tiles of 16 per round (1..16) and tokens per block at most (1..32); 0 = chosen by the
+ * kernel's estimate (the default).  Every shape gives identical bytes; a call that a shape does not fit is
+ * refused with MIND_B200_ERR_INVALID.  Process-wide. */
+int64_t mind_b200_set_w4_shape(int64_t cluster, int64_t row_tiles, int64_t tokens);
+/* The shape that a gemv_w4_* call of these sizes takes (kind as for mind_b200_lcg_fill; experts = 0: one
+ * matrix).  shape_out[7]: blocks per cluster (0: the cross-check kernel runs, everything else 0), row tiles per
+ * round, tokens per block, ring slots, clusters, rounds of all clusters together (of grouped rows: as
+ * estimated), block sizes that were tried.  Without a usable device: what a whole B200 would take. */
+int64_t mind_b200_w4_shape(int64_t kind, int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t experts,
+                           int64_t* shape_out);
 /* Self-test of the bounded waits inside the GEMM kernels: launches a one-warp kernel that waits
  * (with the given limit, 1..1000 ms) on a barrier nothing will ever complete.  The expected
  * result is MIND_B200_ERR_TIMEOUT with the CUDA context still usable. */

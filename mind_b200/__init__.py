@@ -60,13 +60,14 @@ def lib() -> C.CDLL:
                         ("mind_b200_device_count", 0), ("mind_b200_kernel_launches", 0),
                         ("mind_b200_reserve", 2), ("mind_b200_set_gemm_path", 1),
                         ("mind_b200_profile", 1), ("mind_b200_set_devices", 1), ("mind_b200_devices", 0),
-                        ("mind_b200_shutdown", 0), ("mind_b200_set_tile_order", 2),
+                        ("mind_b200_shutdown", 0), ("mind_b200_set_tile_order", 2), ("mind_b200_set_w4_shape", 3),
                         ("mind_b200_rt_deallocate", 1), ("mind_b200_rt_retag", 2), ("mind_b200_rt_synchronize", 0)):
             f = getattr(L, name)
             f.argtypes, f.restype = [i64] * n, i64
         pi64 = C.POINTER(i64)
         L.mind_b200_profile_read.argtypes = [pi64, C.POINTER(C.c_double)]
         L.mind_b200_profile_read.restype = i64
+        L.mind_b200_w4_shape.argtypes, L.mind_b200_w4_shape.restype = [i64] * 6 + [pi64], i64
         L.mind_b200_rt_allocate.argtypes, L.mind_b200_rt_allocate.restype = [i64, pi64, i64, pi64], i64
         L.mind_b200_rt_upload.argtypes, L.mind_b200_rt_upload.restype = [i64, C.c_void_p, i64], i64
         L.mind_b200_rt_download.argtypes, L.mind_b200_rt_download.restype = [i64, C.c_void_p, i64], i64

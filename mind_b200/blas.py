@@ -9,6 +9,8 @@ Nothing here computes: every function forwards to ``libmind_b200.so`` and raises
 """
 from __future__ import annotations
 
+import ctypes as C
+
 import numpy as np
 
 from . import check, last_error, lib, MindB200Error
@@ -210,6 +212,18 @@ def set_gemm_path(path: int) -> None:
 
 def set_tile_order(group_m: int, raster: int = 0) -> None:
     check(lib().mind_b200_set_tile_order(int(group_m), int(raster)))
+
+
+def set_w4_shape(cluster: int = 0, row_tiles: int = 0, tokens: int = 0) -> None:
+    """Shape of the gemv_w4_* kernel, for tests and measurements (0 = chosen by its estimate)."""
+    check(lib().mind_b200_set_w4_shape(int(cluster), int(row_tiles), int(tokens)))
+
+
+def w4_shape(kind: int, m: int, rows: int, cols: int, group: int, experts: int = 0) -> dict:
+    """The shape that a gemv_w4_* call of these sizes takes (kind: KIND_*; experts = 0: one matrix)."""
+    out = (C.c_int64 * 7)()
+    check(lib().mind_b200_w4_shape(kind, m, rows, cols, group, experts, out))
+    return dict(zip(("cluster", "row_tiles", "tokens", "slots", "clusters", "rounds", "tries"), out))
 
 
 def set_devices(count: int) -> None:

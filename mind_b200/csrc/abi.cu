@@ -1067,6 +1067,38 @@ int64_t mind_b200_set_tile_order(int64_t group_m, int64_t raster) {
     return 0;
 }
 
+int64_t mind_b200_set_w4_shape(int64_t cluster, int64_t row_tiles, int64_t tokens) {
+    clear_error();
+    if (cluster < 0 || cluster > 8 || (cluster & (cluster - 1)) || row_tiles < 0 || row_tiles > 16 || tokens < 0 || tokens > 32)
+        return fail(MIND_B200_ERR_INVALID, "cluster must be 0, 1, 2, 4 or 8, row_tiles 0..16, tokens 0..32");
+    tuning().w4_cluster = (int)cluster;
+    tuning().w4_row_tiles = (int)row_tiles;
+    tuning().w4_tokens = (int)tokens;
+    return 0;
+}
+
+int64_t mind_b200_w4_shape(int64_t kind, int64_t m, int64_t rows, int64_t cols, int64_t group, int64_t experts, int64_t* shape_out) {
+    clear_error();
+    if (kind < 0 || kind > 2 || m <= 0 || rows <= 0 || cols <= 0 || experts < 0 || !shape_out)
+        return fail(MIND_B200_ERR_INVALID, "bad argument");
+    if (group <= 0 || group % 32 || group > MAX_DIM) return fail(MIND_B200_ERR_INVALID, "group must be a positive multiple of 32");
+    MB200_TRY(check_experts(experts));
+    if (m > MAX_DIM - 1024 || rows > MAX_DIM - 1024 || cols > MAX_DIM - 1024)
+        return fail(MIND_B200_ERR_TOO_LARGE, "dimension above 2^31-1025");
+    static const int32_t grouped = 0;
+    W4Args a = {};
+    a.kind = kind == 0 ? 2 : (int)kind - 1;
+    a.m = m;
+    a.rows = rows;
+    a.cols = cols;
+    a.group = group;
+    a.experts = experts ? experts : 1;
+    a.offsets = experts ? &grouped : nullptr;  // (whether there are any is all that the choice looks at)
+    DeviceCtx* ctx = usable_device_count() > 0 ? current_ctx() : nullptr;
+    describe_gemv_w4(ctx, a, shape_out);
+    return 0;
+}
+
 int64_t mind_b200_set_devices(int64_t count) {
     clear_error();
     return multi_set_devices(count);

@@ -41,6 +41,9 @@ struct Tuning {
     std::atomic<int> wide_pair{-1};       // int8 GEMM 256 x 512-tile pair kernel: -1 = by shape, 0 = never, 1 = always
     std::atomic<int> group_m{0};          // int8 tile order: m-tiles per group (0 = default)
     std::atomic<int> raster{0};           // int8 tile order variant (0 = default)
+    std::atomic<int> w4_cluster{0};       // gemv_w4: blocks per cluster, row tiles per round, tokens per block
+    std::atomic<int> w4_row_tiles{0};     // (0 = by the estimate)
+    std::atomic<int> w4_tokens{0};
 };
 Tuning& tuning();
 
@@ -303,6 +306,8 @@ struct W4Args {
     int shift, kind;
 };
 int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a);
+// The shape such a call takes on the current device (on a whole B200 where there is none); see mind_b200_w4_shape.
+void describe_gemv_w4(DeviceCtx* ctx, const W4Args& a, int64_t* out);
 struct GroupedArgs {
     const int8_t* a;        // a_rows x k
     const int32_t* rows;    // row of a of every output row, or null: the same row

@@ -65,12 +65,24 @@ gemv_w4_warp_kernel(const W4Args a) {
     }
 }
 
+// What mind_b200_set_w4_shape asks for (0: nothing).
+struct Asked {
+    int cs, rt, tb;
+    bool operator==(const Asked& o) const { return cs == o.cs && rt == o.rt && tb == o.tb; }
+    bool any() const { return cs || rt || tb; }
+};
+Asked asked_shape() {
+    const Tuning& t = tuning();
+    return Asked{t.w4_cluster.load(), t.w4_row_tiles.load(), t.w4_tokens.load()};
+}
+
 // How a call runs on the tensor-core kernel: blocks of at most tb tokens, clusters of cs blocks over the
 // columns, rt row tiles to a round.  Every choice gives the same bytes; the one with the least estimated
 // time is taken.  The estimate is in clocks of the busiest block; its constants were fitted to 33 cases (1 .. 64
 // tokens, 2048 .. 32768 rows, one matrix and 8 .. 128 of them) timed in every shape: the shape taken is 1.3 %
 // slower than the fastest on the geometric mean, 13 % at worst.
-bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
+// fits: clusters of 1, 2, 4 and 8 blocks that the device holds at once.
+bool make_plan(const int (&fits)[4], const Asked& asked, const W4Args& a, int tb, int tc, w4::Plan* out) {
     const int L = a.kind == 0 ? 1 : (a.kind == 1 ? 2 : 4);
     const int ac = tc <= 8 ? 8 : tc, tok8 = (tb + 7) / 8;
     const bool pack = L > 1 && L * tc <= 8;
@@ -96,11 +108,12 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
     double best = 0;
     for (int cs = 1; cs <= 8; cs *= 2) {
         if (cs > kb_total) break;
-        const int fit = w4::cluster_fit(ctx, cs);
-        if (fit < 1) continue;
+        const int fit = fits[cs == 8 ? 3 : cs / 2];
+        if (fit < 1 || (asked.cs && asked.cs != cs)) continue;
         const int kb_slice = (kb_total + cs - 1) / cs;
         const size_t x_bytes = (size_t)kb_slice * w4::KB * L * tc;
         for (int rt = 1; rt <= w4::WARPS; ++rt) {
+            if (asked.rt && asked.rt != rt) continue;
             const int wpr = w4::WARPS / rt, steps = (kb_slice + wpr - 1) / wpr;
             const int64_t row_rounds = (tiles + rt - 1) / rt, rounds = blocks * row_rounds;
             if (rounds > 0x1fffffff) continue;  // (the kernel counts them, at most twice as many, in 32 bits)
@@ -139,6 +152,7 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
                 p.off_x = ring_end + (once ? 0 : (uint32_t)part);
                 p.off_table = p.off_x + (uint32_t)x_bytes;
                 out->grid = (int)(clusters * cs);
+                out->rounds = rounds;
                 out->smem = (int)(1024 + p.off_table + table);
             }
         }
@@ -149,41 +163,55 @@ bool make_plan(DeviceCtx* ctx, const W4Args& a, int tb, int tc, w4::Plan* out) {
 // Tokens per block: all of them up to 32, in blocks of equal size beyond; of grouped rows the kernel
 // learns the groups' sizes itself, and twice the average leaves few experts with a second block.  The
 // choice is a pure function of the sizes, so the last few are kept per thread (it costs as much as a launch).
+bool plan_search(const int (&fits)[4], const Asked& asked, const W4Args& a, w4::Plan* plan, int* tc, int* tries) {
+    int64_t want = a.m;
+    if (a.offsets) {
+        const int64_t twice = 2 * ((a.m + a.experts - 1) / a.experts) + 2;
+        if (want > twice) want = twice;
+    }
+    if (asked.tb && want > asked.tb) want = asked.tb;
+    *tc = *tries = 0;
+    for (int64_t passes = (want + 31) / 32;; ++passes) {  // more blocks where the activations of one would not fit
+        const int tb = (int)((want + passes - 1) / passes);
+        int t = 1;
+        while (t < tb) t *= 2;
+        ++*tries;
+        if (make_plan(fits, asked, a, tb, t, plan)) {
+            *tc = t;
+            return true;
+        }
+        if (tb == 1 || asked.tb) return false;
+    }
+}
+
+void fits_of(DeviceCtx* ctx, int (&fits)[4]) {
+    for (int i = 0; i < 4; ++i) fits[i] = w4::cluster_fit(ctx, 1 << i);
+}
+
 bool plan_for(DeviceCtx* ctx, const W4Args& a, w4::Plan* plan, int* tc) {
     struct Entry {
         int64_t m, rows, cols, group, experts;
         int kind, grouped, device, tc;
+        Asked asked;
         w4::Plan plan;
     };
+    const Asked asked = asked_shape();
     static thread_local Entry cache[8];
     static thread_local int used = 0, next = 0;
     const int grouped = a.offsets ? 1 : 0;
     for (int i = 0; i < used; ++i) {
         const Entry& e = cache[i];
         if (e.m == a.m && e.rows == a.rows && e.cols == a.cols && e.group == a.group && e.experts == a.experts &&
-            e.kind == a.kind && e.grouped == grouped && e.device == ctx->device) {
+            e.kind == a.kind && e.grouped == grouped && e.device == ctx->device && e.asked == asked) {
             *plan = e.plan;
             *tc = e.tc;
             return e.tc != 0;
         }
     }
-    int64_t want = a.m;
-    if (grouped) {
-        const int64_t twice = 2 * ((a.m + a.experts - 1) / a.experts) + 2;
-        if (want > twice) want = twice;
-    }
-    *tc = 0;
-    for (int64_t passes = (want + 31) / 32;; ++passes) {  // more blocks where the activations of one would not fit
-        const int tb = (int)((want + passes - 1) / passes);
-        int t = 1;
-        while (t < tb) t *= 2;
-        if (make_plan(ctx, a, tb, t, plan)) {
-            *tc = t;
-            break;
-        }
-        if (tb == 1) break;
-    }
-    cache[next] = Entry{a.m, a.rows, a.cols, a.group, a.experts, a.kind, grouped, ctx->device, *tc, *plan};
+    int fits[4], tries;
+    fits_of(ctx, fits);
+    plan_search(fits, asked, a, plan, tc, &tries);
+    cache[next] = Entry{a.m, a.rows, a.cols, a.group, a.experts, a.kind, grouped, ctx->device, *tc, asked, *plan};
     next = (next + 1) % 8;
     if (used < 8) ++used;
     return *tc != 0;
@@ -206,12 +234,29 @@ int64_t launch_warp_kernel(DeviceCtx* ctx, const W4Args& a) {
 
 }  // namespace
 
+void describe_gemv_w4(DeviceCtx* ctx, const W4Args& a, int64_t* out) {
+    int fits[4] = {148, 74, 33, 15}, tc, tries;  // of a whole B200
+    if (ctx) fits_of(ctx, fits);
+    w4::Plan plan;
+    const bool found = plan_search(fits, asked_shape(), a, &plan, &tc, &tries);
+    for (int i = 0; i < 6; ++i) out[i] = 0;
+    out[6] = tries;
+    if (!found) return;
+    const w4::Params& p = plan.p;
+    const int64_t shape[6] = {p.cs, p.rt, p.tb, p.slots, plan.grid / p.cs, plan.rounds};
+    for (int i = 0; i < 6; ++i) out[i] = shape[i];
+}
+
 int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
     if (tuning().gemm_path.load() == 1 || a.cols == 0 || a.x_rows == 0) return launch_warp_kernel(ctx, a);
     const int L = a.kind == 0 ? 1 : (a.kind == 1 ? 2 : 4);
     w4::Plan plan;
     int tc = 0;
-    if (!plan_for(ctx, a, &plan, &tc)) return launch_warp_kernel(ctx, a);  // a row of activations too long for eight blocks
+    if (!plan_for(ctx, a, &plan, &tc)) {
+        if (asked_shape().any())
+            return fail(MIND_B200_ERR_INVALID, "the shape that mind_b200_set_w4_shape asks for does not fit this call");
+        return launch_warp_kernel(ctx, a);  // a row of activations too long for eight blocks
+    }
     // TMA reads rows whose pitch and base are multiples of 16 bytes; others are copied to padded rows first
     const int64_t bytes = (a.cols + 1) / 2, pitch = (int64_t)align_up((size_t)bytes, 16);
     const int8_t* w = a.w;

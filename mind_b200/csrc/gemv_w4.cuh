@@ -617,6 +617,7 @@ __global__ void __launch_bounds__(THREADS, 1) gemv_w4_mma_kernel(const __grid_co
 struct Plan {
     Params p;
     int grid, smem;
+    int64_t rounds;  // of all clusters together (of grouped rows: as estimated)
 };
 
 template <int L, int TC, int GB>

@@ -801,3 +801,125 @@ def test_gemv_w4_slots_are_refilled_behind_their_readers(torch_gpu, gpu, kind, t
         wrong += (y != want[n % sets]).sum()
     gpu.synchronize()
     assert int(wrong) == 0
+
+
+# ------------------------------------------------------- shapes of the 4-bit kernel, asked for by name
+@pytest.fixture
+def w4_shape():
+    yield blas.set_w4_shape
+    blas.set_w4_shape()
+
+
+def test_w4_shape_refuses(w4_shape):
+    for bad in ((3, 0, 0), (16, 0, 0), (-1, 0, 0), (0, 17, 0), (0, -1, 0), (0, 0, 33), (0, 0, -1)):
+        refused(mind_b200.ERR_INVALID, w4_shape, *bad)
+    for bad in ((3, 1, 1, 32, 32), (0, 0, 1, 32, 32), (0, 1, 0, 32, 32), (0, 1, 1, 0, 32), (0, 1, 1, 32, 48), (0, 1, 1, 32, 32, -1)):
+        refused(mind_b200.ERR_INVALID, blas.w4_shape, *bad)
+    refused(mind_b200.ERR_TOO_LARGE, blas.w4_shape, 0, 1, 1, 32, 32, 4097)
+    refused(mind_b200.ERR_TOO_LARGE, blas.w4_shape, 0, 1, 1 << 31, 32, 32)
+
+
+def test_w4_shape_is_what_was_asked_for(w4_shape):
+    for kind in (blas.KIND_I8, blas.KIND_I16, blas.KIND_Q16):
+        for experts in (0, 8):
+            free = blas.w4_shape(kind, 24, 5000, 4608, 128, experts)
+            assert free["cluster"] in (1, 2, 4, 8) and 1 <= free["row_tiles"] <= 16 and 2 <= free["slots"] <= 8
+            for cs, rt, tb in ((1, 5, 2), (2, 16, 0), (4, 0, 3), (8, 1, 1)):
+                w4_shape(cs, rt, tb)
+                got = blas.w4_shape(kind, 24, 5000, 4608, 128, experts)
+                assert got["cluster"] == cs and got["row_tiles"] == (rt or got["row_tiles"])
+                assert got["tokens"] == (tb or got["tokens"]) and got["rounds"] >= got["clusters"] >= 1
+            w4_shape()
+            assert blas.w4_shape(kind, 24, 5000, 4608, 128, experts) == free
+    w4_shape(8, 0, 0)  # fewer than eight units of 512 columns
+    assert blas.w4_shape(blas.KIND_I8, 1, 100, 1024, 32)["cluster"] == 0
+
+
+@pytest.mark.gpu
+def test_a_shape_that_does_not_fit_is_refused(gpu, w4_shape):
+    w, s, x, y = np.zeros((16, 512), np.int8), np.zeros((16, 32), np.int16), np.zeros(1024, np.int8), np.zeros(16, I32)
+    w4_shape(8, 0, 0)
+    refused(mind_b200.ERR_INVALID, gpu.gemv_w4_i8, w, s, x, y, 1, 16, 1024, 32, 0)
+    w4_shape()
+    assert gpu.gemv_w4_i8(w, s, x, y, 1, 16, 1024, 32, 0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["i8", "i16", "q16"])
+@pytest.mark.parametrize("cs", [1, 2, 4, 8])
+@pytest.mark.parametrize("rt", [1, 3, 5, 6, 16])
+def test_gemv_w4_rounds(torch_gpu, gpu, w4_shape, kind, cs, rt):
+    """Every cluster size and several row tiles with three or more rounds to a cluster: the ring and the sums are
+    carried from one round to the next, activations change in between.  Against the cross-check kernel, and some rows
+    against numpy.  Odd rows; odd columns (rows that have to be laid out) and whole ones; one matrix and grouped rows."""
+    torch = torch_gpu
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(cs * 100 + rt)
+
+    def some(shape, bits, dtype):
+        return torch.randint(-2 ** (bits - 1), 2 ** (bits - 1), shape, generator=gen, device="cuda", dtype=torch.int64).to(dtype)
+
+    bits, dtype = {"i8": (8, torch.int8), "i16": (16, torch.int16), "q16": (32, torch.int32)}[kind]
+    code = {"i8": blas.KIND_I8, "i16": blas.KIND_I16, "q16": blas.KIND_Q16}[kind]
+    # tokens whose activations fit beside the ring
+    wide = {"i8": 12, "i16": 4 if cs == 1 else 12, "q16": {1: 4, 2: 7}.get(cs, 12)}[kind]
+    for tb, cols, group, experts in ((1, 4608, 128, 0), (wide, 4389, 32, 0), (3, 4096 + 160, 64, 0), (2, 4100, 96, 4), (wide, 4608, 32, 4)):
+        blocks = 6
+        row_rounds = 3 * (148 // cs) // blocks + 1
+        rows = 16 * rt * row_rounds - 5
+        m = blocks * tb
+        stack, groups = (experts or 1, rows), -(-cols // group)
+        w = torch.randint(-128, 128, (*stack, (cols + 1) // 2), generator=gen, device="cuda", dtype=torch.int16).to(torch.int8)
+        s, x = some((*stack, groups), 16, torch.int16), some((m, cols), bits, dtype)
+        y, want = (torch.full((m, rows), CANARY, dtype=torch.int32, device="cuda") for _ in range(2))
+        if experts:  # sizes that fill some blocks of tokens and not others
+            offsets = torch.tensor([0, m // 2 + 1, m // 2 + 1, m - 1, m], dtype=torch.int32, device="cuda")
+            rows_of = torch.randint(-1, m + 1, (m,), generator=gen, device="cuda", dtype=torch.int32)
+
+        def call(out):
+            if experts:
+                getattr(gpu, f"gemv_w4_grouped_{kind}")(w, s, x, rows_of, offsets, out, m, rows, cols, group, 13, experts, m)
+            else:
+                getattr(gpu, f"gemv_w4_{kind}")(w, s, x, out, m, rows, cols, group, 13)
+
+        gpu.set_gemm_path(1)
+        call(want)
+        gpu.set_gemm_path(0)
+        w4_shape(cs, rt, tb)
+        shape = gpu.w4_shape(code, m, rows, cols, group, experts)
+        assert shape["cluster"] == cs and shape["row_tiles"] == rt and shape["rounds"] >= 3 * shape["clusters"], shape
+        call(y)
+        w4_shape()
+        call_differs = int((y != want).sum())
+        assert call_differs == 0, (tb, cols, group, experts, call_differs)
+        r = np.unique(np.concatenate([[0, rows - 1], np.random.default_rng(rt).integers(0, rows, 6)]))
+        xs = x.cpu().numpy()
+        for e in range(experts or 1):
+            lo, hi = (int(offsets[e]), int(offsets[e + 1])) if experts else (0, m)
+            if hi > lo:
+                xe = gather(xs, rows_of.cpu().numpy(), np.arange(lo, hi), cols) if experts else xs
+                assert np.array_equal(y[lo:hi].cpu().numpy()[:, r], ref_w4(w[e].cpu().numpy()[r], s[e].cpu().numpy()[r], xe, cols, group, 13))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind,m,rows,cols,group", [("i8", 300, 4100, 4097, 128), ("q16", 70, 8192, 8192, 32), ("i16", 41, 20000, 5120, 64)])
+def test_gemv_w4_many_tokens_by_the_estimate(torch_gpu, gpu, kind, m, rows, cols, group):
+    """Shapes of several rounds that the kernel takes of its own accord."""
+    torch = torch_gpu
+    rng = np.random.default_rng(m)
+    code = {"i8": blas.KIND_I8, "i16": blas.KIND_I16, "q16": blas.KIND_Q16}[kind]
+    shape = gpu.w4_shape(code, m, rows, cols, group)
+    assert shape["rounds"] > shape["clusters"], shape
+    w, s, x = w4_of(rng, rows, (cols + 1) // 2), scale_of(rng, rows, -(-cols // group)), x_of(rng, kind, (m, cols))
+    dw, ds, dx = dev(torch, w, s, x)
+    y, want = (torch.full((m, rows), CANARY, dtype=torch.int32, device="cuda") for _ in range(2))
+    fn = getattr(gpu, f"gemv_w4_{kind}")
+    gpu.set_gemm_path(1)
+    fn(dw, ds, dx, want, m, rows, cols, group, 5)
+    gpu.set_gemm_path(0)
+    for _ in range(3):
+        y.fill_(CANARY)
+        fn(dw, ds, dx, y, m, rows, cols, group, 5)
+        assert torch.equal(y, want)
+    r = rng.integers(0, rows, 8)
+    assert np.array_equal(y.cpu().numpy()[:, r], ref_w4(w[r], s[r], x, cols, group, 5))
