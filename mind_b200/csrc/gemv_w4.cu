@@ -171,7 +171,10 @@ bool plan_search(const int (&fits)[4], const Asked& asked, const W4Args& a, w4::
     }
     if (asked.tb && want > asked.tb) want = asked.tb;
     *tc = *tries = 0;
-    for (int64_t passes = (want + 31) / 32;; ++passes) {  // more blocks where the activations of one would not fit
+    // More blocks where the activations of one would not fit.  What fits goes by the power of two above tb, so only
+    // those are tried: six at most, whatever the number of tokens.
+    for (int64_t most = 32;;) {
+        const int64_t passes = (want + most - 1) / most;
         const int tb = (int)((want + passes - 1) / passes);
         int t = 1;
         while (t < tb) t *= 2;
@@ -181,6 +184,7 @@ bool plan_search(const int (&fits)[4], const Asked& asked, const W4Args& a, w4::
             return true;
         }
         if (tb == 1 || asked.tb) return false;
+        most = t / 2;
     }
 }
 

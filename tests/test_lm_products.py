@@ -923,3 +923,12 @@ def test_gemv_w4_many_tokens_by_the_estimate(torch_gpu, gpu, kind, m, rows, cols
         assert torch.equal(y, want)
     r = rng.integers(0, rows, 8)
     assert np.array_equal(y.cpu().numpy()[:, r], ref_w4(w[r], s[r], x, cols, group, 5))
+
+
+def test_w4_shape_is_found_in_a_few_tries():
+    """The host's search must not grow with the number of tokens: it runs inside the call, under the device's lock."""
+    for m in (1, 33, 4097, 1_000_000, 2 ** 31 - 1025):
+        for cols in (32, 28672, 200_000, 400_000, 3_000_000):
+            for kind in (blas.KIND_I8, blas.KIND_I16, blas.KIND_Q16):
+                for experts in (0, 5):
+                    assert 1 <= blas.w4_shape(kind, m, 4096, cols, 128, experts)["tries"] <= 6, (m, cols, kind, experts)
