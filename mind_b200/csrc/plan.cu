@@ -244,7 +244,7 @@ int64_t launch_expert_plan(DeviceCtx* ctx, const int32_t* ids, int32_t* offsets,
     // Blocks of the two-launch form: what keeps the table of totals, which every block reads, small.
     int64_t wide = 80000 / experts;
     if (wide > ctx->sm_count) wide = ctx->sm_count;
-    const bool two = count > 16384 && wide > 2 * MAX_CLUSTER;
+    const bool two = count > 16384;
     int blocks = 1;
     if (!two) {
         // Blocks of eight warps with one group of 32 each while that lasts (8192 ids over 64 experts: 4.8 us, of
