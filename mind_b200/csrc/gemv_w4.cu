@@ -276,7 +276,7 @@ int64_t launch_gemv_w4(DeviceCtx* ctx, const W4Args& a) {
     w4::Params& p = plan.p;
     p.a = a;
     p.groups = (int)((a.cols + a.group - 1) / a.group);
-    p.group32 = (int)(a.group / 32 > 0x3fffffff ? 0x40000000 : a.group / 32);
+    p.group32 = (int)(a.group / 32);
     const int gb = p.group32 % 4 == 0 ? 4 : (p.group32 % 2 == 0 ? 2 : 1), ns = w4::KB / 128 / gb;
     p.group_shift = -1;
     for (int i = 0; i < 31; ++i)
