@@ -20,21 +20,19 @@ def addr(x) -> int:
     """Raw address of a numpy array, a torch tensor, or an int passed through."""
     if type(x) is int:
         return x
-    try:  # tensors first: launch-bound callers pass several per call
+    if isinstance(x, np.ndarray):
+        if not x.flags["C_CONTIGUOUS"]:
+            raise ValueError("operands must be C-contiguous")
+        return x.ctypes.data
+    try:  # (launch-bound callers pass several tensors per call)
         if x.is_contiguous():
             return x.data_ptr()
     except AttributeError:
         pass
     if isinstance(x, (int, np.integer)):
         return int(x)
-    if isinstance(x, np.ndarray):
-        if not x.flags["C_CONTIGUOUS"]:
-            raise ValueError("operands must be C-contiguous")
-        return x.ctypes.data
     if hasattr(x, "data_ptr"):
-        if not x.is_contiguous():
-            raise ValueError("operands must be contiguous")
-        return x.data_ptr()
+        raise ValueError("operands must be contiguous")
     raise TypeError(f"cannot take the address of {type(x)!r}")
 
 

@@ -932,3 +932,23 @@ def test_w4_shape_is_found_in_a_few_tries():
             for kind in (blas.KIND_I8, blas.KIND_I16, blas.KIND_Q16):
                 for experts in (0, 5):
                     assert 1 <= blas.w4_shape(kind, m, 4096, cols, 128, experts)["tries"] <= 6, (m, cols, kind, experts)
+
+
+def test_addresses_of_operands():
+    """Each kind of operand is recognised for what it is: an array is not first asked for a tensor's methods."""
+    class Array(np.ndarray):
+        def __getattr__(self, name):
+            raise AssertionError(f"looked for {name}")
+
+    a = np.arange(12, dtype=I32).reshape(3, 4)
+    assert blas.addr(a.view(Array)) == blas.addr(a) == a.ctypes.data
+    assert blas.addr(7) == 7 and blas.addr(np.int64(9)) == 9 and blas.addr(True) == 1
+    with pytest.raises(ValueError):
+        blas.addr(a.T)
+    with pytest.raises(TypeError):
+        blas.addr("a")
+    torch = pytest.importorskip("torch")
+    t = torch.zeros(3, 4)
+    assert blas.addr(t) == t.data_ptr()
+    with pytest.raises(ValueError):
+        blas.addr(t.t())
