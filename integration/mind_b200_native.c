@@ -20,7 +20,10 @@
  * There is no CPU fallback on purpose: a caller that wants the CPU kernels simply does not
  * list this file.
  *
- * Plain C99 + POSIX (dlopen, pthread_once); no CUDA headers are needed to compile it.
+ * A library older than the products of quantised language models serves everything else; those
+ * return -3 with it.
+ *
+ * C99 + POSIX (dlopen, pthread_once) + __thread; no CUDA headers are needed to compile it.
  */
 #include <dlfcn.h>
 #include <pthread.h>
@@ -64,6 +67,9 @@ static void *b200_sym(const char *name) {
     return p;
 }
 
+/* A name that older libraries lack: only calls of it are refused then. */
+static void *b200_newer_sym(const char *name) { return dlsym(g_b200.handle, name); }
+
 static void b200_load(void) {
     const char *path = getenv("MIND_B200_LIB");
     if (!path || !*path) path = "libmind_b200.so";
@@ -84,28 +90,39 @@ static void b200_load(void) {
     g_b200.dot_q16 = (fn3_t)b200_sym("__mind_blas_dot_q16_v");
     g_b200.dot_l1_q16 = (fn3_t)b200_sym("__mind_blas_dot_l1_q16_v");
     g_b200.dot_i16 = (fn3_t)b200_sym("__mind_blas_dot_i16_v");
-    g_b200.w4_i8 = (fn9_t)b200_sym("__mind_b200_gemv_w4_i8");
-    g_b200.w4_i16 = (fn9_t)b200_sym("__mind_b200_gemv_w4_i16");
-    g_b200.w4_q16 = (fn9_t)b200_sym("__mind_b200_gemv_w4_q16");
-    g_b200.w4_grouped_i8 = (fn13_t)b200_sym("__mind_b200_gemv_w4_grouped_i8");
-    g_b200.w4_grouped_i16 = (fn13_t)b200_sym("__mind_b200_gemv_w4_grouped_i16");
-    g_b200.w4_grouped_q16 = (fn13_t)b200_sym("__mind_b200_gemv_w4_grouped_q16");
-    g_b200.mm_grouped_i8 = (fn12_t)b200_sym("__mind_b200_matmul_grouped_i8");
-    g_b200.mm_grouped_i8_bt = (fn12_t)b200_sym("__mind_b200_matmul_grouped_i8_bt");
-    g_b200.expert_plan = (fn7_t)b200_sym("__mind_b200_expert_plan");
+    g_b200.w4_i8 = (fn9_t)b200_newer_sym("__mind_b200_gemv_w4_i8");
+    g_b200.w4_i16 = (fn9_t)b200_newer_sym("__mind_b200_gemv_w4_i16");
+    g_b200.w4_q16 = (fn9_t)b200_newer_sym("__mind_b200_gemv_w4_q16");
+    g_b200.w4_grouped_i8 = (fn13_t)b200_newer_sym("__mind_b200_gemv_w4_grouped_i8");
+    g_b200.w4_grouped_i16 = (fn13_t)b200_newer_sym("__mind_b200_gemv_w4_grouped_i16");
+    g_b200.w4_grouped_q16 = (fn13_t)b200_newer_sym("__mind_b200_gemv_w4_grouped_q16");
+    g_b200.mm_grouped_i8 = (fn12_t)b200_newer_sym("__mind_b200_matmul_grouped_i8");
+    g_b200.mm_grouped_i8_bt = (fn12_t)b200_newer_sym("__mind_b200_matmul_grouped_i8_bt");
+    g_b200.expert_plan = (fn7_t)b200_newer_sym("__mind_b200_expert_plan");
     g_b200.last_error = (err_t)b200_sym("mind_b200_last_error");
 }
 
+static __thread const char *t_b200_lacks; /* what this thread's last call was refused for, or NULL */
+
 static int b200_ready(void) {
     pthread_once(&g_b200_once, b200_load);
+    t_b200_lacks = NULL;
     return g_b200.handle && !g_b200.load_error[0];
 }
+
+static int b200_lacks(const char *why) {
+    t_b200_lacks = why;
+    return 0;
+}
+#define B200_HAS(name, slot) \
+    (b200_ready() && (g_b200.slot || b200_lacks("libmind_b200: this library is older than " #name)))
 
 /* Why the last call of this thread's library failed, or why the library could not be loaded;
  * NULL when there is nothing to report. */
 const char *mind_b200_native_last_error(void) {
     pthread_once(&g_b200_once, b200_load);
     if (g_b200.load_error[0]) return g_b200.load_error;
+    if (t_b200_lacks) return t_b200_lacks;
     return g_b200.last_error ? g_b200.last_error() : NULL;
 }
 
@@ -139,21 +156,22 @@ FORWARD3(__mind_blas_dot_i16_v, dot_i16)
 
 /* products of quantised language models: no counterpart in the reference (new names) */
 #define FORWARD13(name, slot)                                                                                        \
-    int64_t name(int64_t w, int64_t s, int64_t x, int64_t r, int64_t o, int64_t y, int64_t m, int64_t rows,           \
+    int64_t name(int64_t w, int64_t s, int64_t x, int64_t r, int64_t o, int64_t y, int64_t m, int64_t rows,          \
                  int64_t cols, int64_t group, int64_t shift, int64_t experts, int64_t x_rows) {                      \
-        return b200_ready() ? g_b200.slot(w, s, x, r, o, y, m, rows, cols, group, shift, experts, x_rows)            \
-                            : MIND_B200_NATIVE_NO_LIBRARY;                                                           \
+        return B200_HAS(name, slot) ? g_b200.slot(w, s, x, r, o, y, m, rows, cols, group, shift, experts, x_rows)    \
+                                    : MIND_B200_NATIVE_NO_LIBRARY;                                                   \
     }
 #define FORWARD12(name, slot)                                                                                        \
-    int64_t name(int64_t a, int64_t r, int64_t b, int64_t o, int64_t s, int64_t c, int64_t m, int64_t k, int64_t n,   \
+    int64_t name(int64_t a, int64_t r, int64_t b, int64_t o, int64_t s, int64_t c, int64_t m, int64_t k, int64_t n,  \
                  int64_t experts, int64_t a_rows, int64_t shift) {                                                   \
-        return b200_ready() ? g_b200.slot(a, r, b, o, s, c, m, k, n, experts, a_rows, shift)                         \
-                            : MIND_B200_NATIVE_NO_LIBRARY;                                                           \
+        return B200_HAS(name, slot) ? g_b200.slot(a, r, b, o, s, c, m, k, n, experts, a_rows, shift)                 \
+                                    : MIND_B200_NATIVE_NO_LIBRARY;                                                   \
     }
 #define FORWARD9(name, slot)                                                                                         \
-    int64_t name(int64_t w, int64_t s, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols,              \
+    int64_t name(int64_t w, int64_t s, int64_t x, int64_t y, int64_t tokens, int64_t rows, int64_t cols,             \
                  int64_t group, int64_t shift) {                                                                     \
-        return b200_ready() ? g_b200.slot(w, s, x, y, tokens, rows, cols, group, shift) : MIND_B200_NATIVE_NO_LIBRARY; \
+        return B200_HAS(name, slot) ? g_b200.slot(w, s, x, y, tokens, rows, cols, group, shift)                      \
+                                    : MIND_B200_NATIVE_NO_LIBRARY;                                                   \
     }
 FORWARD9(__mind_b200_gemv_w4_i8, w4_i8)
 FORWARD9(__mind_b200_gemv_w4_i16, w4_i16)
@@ -165,5 +183,7 @@ FORWARD12(__mind_b200_matmul_grouped_i8, mm_grouped_i8)
 FORWARD12(__mind_b200_matmul_grouped_i8_bt, mm_grouped_i8_bt)
 int64_t __mind_b200_expert_plan(int64_t ids, int64_t offsets, int64_t rows, int64_t place, int64_t count, int64_t experts,
                                 int64_t per) {
-    return b200_ready() ? g_b200.expert_plan(ids, offsets, rows, place, count, experts, per) : MIND_B200_NATIVE_NO_LIBRARY;
+    return B200_HAS(__mind_b200_expert_plan, expert_plan)
+               ? g_b200.expert_plan(ids, offsets, rows, place, count, experts, per)
+               : MIND_B200_NATIVE_NO_LIBRARY;
 }

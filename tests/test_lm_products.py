@@ -952,3 +952,52 @@ def test_addresses_of_operands():
     assert blas.addr(t) == t.data_ptr()
     with pytest.raises(ValueError):
         blas.addr(t.t())
+
+
+OLDER_LIBRARY = """
+#include <stdint.h>
+typedef int64_t i;
+#define SIX(n, v) i n(i a, i b, i c, i d, i e, i f) { (void)a, (void)b, (void)c, (void)d, (void)e, (void)f; return v; }
+#define FIVE(n, v) i n(i a, i b, i c, i d, i e) { (void)a, (void)b, (void)c, (void)d, (void)e; return v; }
+#define THREE(n, v) i n(i a, i b, i c) { (void)a, (void)b, (void)c; return v; }
+SIX(__mind_blas_matmul_mm_i8_v, 1) SIX(__mind_blas_matmul_mm_i8_mt_v, 2) SIX(__mind_blas_matmul_mm_q16_v, 3)
+SIX(__mind_blas_matmul_mm_q16_mt_v, 4) SIX(__mind_b200_matmul_mm_i16, 5)
+FIVE(__mind_blas_gemv_q16_mt, 6) FIVE(__mind_blas_matmul_rmajor_q16_v, 7) FIVE(__mind_blas_matmul_rmajor_i16_v, 8)
+THREE(__mind_blas_dot_q16_v, 9) THREE(__mind_blas_dot_l1_q16_v, 10) THREE(__mind_blas_dot_i16_v, 11)
+const char *mind_b200_last_error(void) { return "the older library's own"; }
+"""
+OLDER_CHILD = r"""
+import ctypes as C, sys
+L = C.CDLL(sys.argv[1])
+i64 = C.c_int64
+def call(name, n):
+    f = getattr(L, name); f.argtypes, f.restype = [i64] * n, i64
+    return f(*[0] * n)
+err = L.mind_b200_native_last_error; err.restype = C.c_char_p
+for want, (name, n) in enumerate([("__mind_blas_matmul_mm_i8_v", 6), ("__mind_blas_matmul_mm_i8_mt_v", 6), ("__mind_blas_matmul_mm_q16_v", 6),
+        ("__mind_blas_matmul_mm_q16_mt_v", 6), ("__mind_b200_matmul_mm_i16", 6), ("__mind_blas_gemv_q16_mt", 5),
+        ("__mind_blas_matmul_rmajor_q16_v", 5), ("__mind_blas_matmul_rmajor_i16_v", 5), ("__mind_blas_dot_q16_v", 3),
+        ("__mind_blas_dot_l1_q16_v", 3), ("__mind_blas_dot_i16_v", 3)], 1):
+    assert call(name, n) == want, (name, err())
+assert err() == b"the older library's own"
+for n, names in {9: ["gemv_w4_i8", "gemv_w4_i16", "gemv_w4_q16"], 7: ["expert_plan"], 12: ["matmul_grouped_i8", "matmul_grouped_i8_bt"],
+                 13: ["gemv_w4_grouped_i8", "gemv_w4_grouped_i16", "gemv_w4_grouped_q16"]}.items():
+    for name in names:
+        assert call("__mind_b200_" + name, n) == -3, name
+        assert b"__mind_b200_" + name.encode() in err(), (name, err())
+assert call("__mind_blas_matmul_mm_i8_v", 6) == 1 and err() == b"the older library's own"
+print("ok")
+"""
+
+
+def test_native_sources_file_with_an_older_library(tmp_path):
+    """A library that lacks the products of quantised language models serves everything else as before."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    shim, old = str(tmp_path / "libshim.so"), str(tmp_path / "libmind_b200.so")
+    (tmp_path / "old.c").write_text(OLDER_LIBRARY)
+    for out, src, libs in ((shim, os.path.join(root, "integration", "mind_b200_native.c"), ["-ldl", "-lpthread"]),
+                           (old, str(tmp_path / "old.c"), [])):
+        subprocess.run(["gcc", "-O2", "-Wall", "-Wextra", "-Werror", "-fPIC", "-shared", "-o", out, src, *libs], check=True)
+    r = subprocess.run([sys.executable, "-c", OLDER_CHILD, shim], capture_output=True, text=True, timeout=300,
+                       env=dict(os.environ, MIND_B200_LIB=old))
+    assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
