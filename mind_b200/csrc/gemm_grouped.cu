@@ -438,7 +438,8 @@ gemm_grouped_tc_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_co
             const uint32_t t0 = tmem_base + ((uint32_t)(q * 32) << 16) + as * BLOCK_N;
             const int32_t* const scale = p.scale ? p.scale + (size_t)t.e * p.n : nullptr;
             int f_next = scale && col_tile + lane < p.n ? __ldg(scale + col_tile + lane) : 0;
-            if (!wait_bounded(tfull0 + 8 * as, aph, abort_s, p.err, 4)) break;
+            // (all lanes give up together: what follows is done by whole warps)
+            if (!__all_sync(0xffffffffu, wait_bounded(tfull0 + 8 * as, aph, abort_s, p.err, 4))) break;
             tc_fence_after();
             for (int c0 = 0; c0 < BLOCK_N && valid > 0; c0 += 32) {
                 const int col = col_tile + c0;
