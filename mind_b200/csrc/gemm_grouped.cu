@@ -14,8 +14,9 @@
 // expert, and tile i of that list goes to CTA i mod grid.  A tile never spans two experts, so its
 // last rows may belong to the next one: they are multiplied and not stored.
 //
-// What bounds it.  Few rows an expert: the weights (64 experts, 128 rows, 2048 x 2816, gathered: 52 us a call;
-// ncu: 249 MB read, all of the weights in use).  Many: the tensor pipe under the power cap (32768 x 4096 x
+// What bounds it.  Few rows an expert: the weights (64 experts, 128 gathered rows, 2048 x 2816: 47 to 53 us a
+// call; about 41 experts get a row, whose 241 MB would take 37 us: ncu shows no byte read twice, at 4.3 TB/s in
+// the product itself).  Many: the tensor pipe under the power cap (32768 x 4096 x
 // 4096 over 16 experts: 390 us = 2.82 POP/s in a burst, the dense kernel's rate at that size; 516 us back to
 // back with rows gathered, of which their copy is 45).  Between: whole waves of tiles.
 #include "common.h"

@@ -79,8 +79,9 @@ Asked asked_shape() {
 // How a call runs on the tensor-core kernel: blocks of at most tb tokens, clusters of cs blocks over the
 // columns, rt row tiles to a round.  Every choice gives the same bytes; the one with the least estimated
 // time is taken.  The estimate is in clocks of the busiest block; its constants were fitted to 33 cases (1 .. 64
-// tokens, 2048 .. 32768 rows, one matrix and 8 .. 128 of them) timed in every shape: the shape taken is 1.3 %
-// slower than the fastest on the geometric mean, 13 % at worst.
+// tokens, 1024 .. 32768 rows, one matrix and 8 .. 128 of them) timed in every shape that fits (as
+// mind_b200_set_w4_shape asks for them): the shape taken is 1.2 % slower than the fastest on the geometric mean,
+// 9 % at worst (int16, 8 tokens through 4 of 32 experts of 2048 x 4096: 31.0 against 28.5 us).
 // fits: clusters of 1, 2, 4 and 8 blocks that the device holds at once.
 bool make_plan(const int (&fits)[4], const Asked& asked, const W4Args& a, int tb, int tc, w4::Plan* out) {
     const int L = a.kind == 0 ? 1 : (a.kind == 1 ? 2 : 4);

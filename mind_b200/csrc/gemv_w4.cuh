@@ -24,11 +24,12 @@
 //   across the cluster by remote reads: integer sums, so no order changes a bit, and nothing is kept in
 //   global memory.
 //
-// What bounds it.  One or two tokens: memory behind a set-up of about 5 us (28672 x 8192 int8: 24.7 to 25.8
-// us a call, 4.8 TB/s of weights and scales, 0.73 of the copy bandwidth; 4096 x 4096: 6.2 us, of which the host
-// needs about as much to make the call).  More: the latency of the main loop on four warps a scheduler (8192 x
-// 8192 Q16.16, eight tokens, groups of 32: 22.8 us against 5.9 us of memory time; no pipe is more than half
-// busy).  MMAs run at 8.2 clocks a scheduler whatever their operands.
+// What bounds it.  One or two tokens: memory behind a set-up of about 5 us (28672 x 8192 int8: 24.9 to 26.0
+// us a call, 4.8 TB/s of weights and scales, 0.73 of the copy bandwidth; int16 and Q16.16 31 us; 4096 x 4096
+// Q16.16: 6.4 us, of which the host needs about as much to make the call).  More: the latency of the main loop
+// on four warps a scheduler (8192 x 8192 Q16.16, eight tokens, groups of 32: 22.4 us against 5.9 us of memory
+// time; 0.44 instructions a clock and scheduler, no pipe more than half busy).  MMAs run at 8.2 clocks a
+// scheduler whatever their operands.
 #pragma once
 #include "common.h"
 #include "ptx.cuh"
